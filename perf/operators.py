@@ -484,7 +484,7 @@ def exact(case, seed):
                     y = (y / step).round() * step
                 values.append((y * now[:, None, None]).transpose(0, 1))
                 scale[p] = now
-                out[name], out[name + "_scale"] = torch.cat(values), scale
+            out[name], out[name + "_scale"] = torch.cat(values), scale
         return out
     q, group = s["q"].to(f64), c["q_heads"] // c["kv_heads"]
     out = torch.empty_like(q)
