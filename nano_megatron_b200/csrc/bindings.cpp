@@ -114,6 +114,22 @@ void cp_reduce(at::Tensor acc, std::vector<int64_t> slots_even, std::vector<int6
                int64_t mask, int64_t flags_ptr, int64_t epoch_ptr, at::Tensor status);
 void scale_inplace(at::Tensor x, double s);
 void dropout_apply(at::Tensor x, at::Tensor y, double p, int64_t seed);
+std::vector<at::Tensor> plan_step(at::Tensor context, at::Tensor fresh, at::Tensor tables,
+                                  at::Tensor free_pages, at::Tensor free_count, int64_t page_size,
+                                  int64_t num_tokens);
+void append_kv(at::Tensor k_pages, at::Tensor v_pages, at::Tensor k_scale, at::Tensor v_scale,
+               at::Tensor k, at::Tensor v, at::Tensor touched);
+std::vector<at::Tensor> read_kv(at::Tensor k_pages, at::Tensor v_pages, at::Tensor k_scale,
+                                at::Tensor v_scale, at::Tensor slots);
+at::Tensor paged_attention(at::Tensor q, at::Tensor k_pages, at::Tensor v_pages,
+                           at::Tensor k_scale, at::Tensor v_scale, at::Tensor tables,
+                           at::Tensor q_starts, at::Tensor kv_lens, int64_t max_new,
+                           double softmax_scale, c10::optional<at::Tensor> lse,
+                           at::Tensor status);
+at::Tensor adjust_logits(at::Tensor logits, at::Tensor history, at::Tensor lens, at::Tensor prompts,
+                         c10::optional<at::Tensor> repetition, c10::optional<at::Tensor> presence,
+                         c10::optional<at::Tensor> frequency, c10::optional<at::Tensor> bias_ids,
+                         c10::optional<at::Tensor> bias, c10::optional<at::Tensor> allowed);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "nano_megatron_b200 sm_100a kernels (tcgen05 GEMM, flash attention, fused ops)";
@@ -209,6 +225,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("cp_pull", &cp_pull, "CP ring: pull a peer's published block into local memory");
   m.def("cp_push", &cp_push, "CP ring: store a dK/dV partial into its owner's return slot");
   m.def("cp_reduce", &cp_reduce, "CP ring: add the returned partials once every rank signalled");
+  m.def("plan_step", &plan_step, "batched serving: row starts, positions, slots, touched pages");
+  m.def("append_kv", &append_kv, "quantise new K/V rows into the 8-bit paged cache");
+  m.def("read_kv", &read_kv, "cached K/V rows as bf16 values");
+  m.def("paged_attention", &paged_attention, "attention over the 8-bit paged cache");
+  m.def("adjust_logits", &adjust_logits, "penalties, bias and allow-mask on logits");
   m.def("launch_count", []() { return nmb::launch_counter().load(); },
         "number of kernel launches issued by this library so far (graph replays included)");
   m.def("record_graph_launches", [](int64_t n) { nmb::launch_counter() += n; },

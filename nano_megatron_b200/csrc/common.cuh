@@ -49,6 +49,7 @@ enum StatusCode : int {
   kStatusGemmMmaTimeout = 0x102,
   kStatusGemmEpilogueTimeout = 0x103,
   kStatusAttnTimeout = 0x201,
+  kStatusSmemAlignment = 0x202,
   kStatusPeerFlagTimeout = 0x301,
   kStatusPeerBarrierTimeout = 0x302,
   kStatusReplicaFlagTimeout = 0x401,
