@@ -61,14 +61,7 @@ __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) 
   return lo | (hi << 16);
 }
 
-// Two codes (bytes 0 and 1 of `v`) as f16x2; both formats fit f16 exactly.
-__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint16_t v) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(v));
-  return r;
-}
-
-// Four codes as two f16x2 (bytes 0,1 and 2,3). int8: a byte c ^ 0x80 in the low mantissa bits
+// Four codes as two f16x2 (bytes 0,1 and 2,3), exact in both formats. int8: a byte c ^ 0x80 in the low mantissa bits
 // of 1024 gives 1024 + 128 + c exactly; subtract 1152.
 template <bool INT8>
 __device__ __forceinline__ void decode4(uint32_t v, uint32_t& lo, uint32_t& hi) {
@@ -81,8 +74,10 @@ __device__ __forceinline__ void decode4(uint32_t v, uint32_t& lo, uint32_t& hi) 
     lo = *reinterpret_cast<uint32_t*>(&ha);
     hi = *reinterpret_cast<uint32_t*>(&hb);
   } else {
-    lo = e4m3x2_to_f16x2(static_cast<uint16_t>(v));
-    hi = e4m3x2_to_f16x2(static_cast<uint16_t>(v >> 16));
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(v));
   }
 }
 

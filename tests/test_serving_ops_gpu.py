@@ -302,6 +302,13 @@ def test_decode_one_request(page, n):
     _check([n], [1], 2, 2, 64, page, INT8)
 
 
+@pytest.mark.parametrize("dtype", [E4M3, INT8])
+@pytest.mark.parametrize("D,Hq,H,page", [(128, 32, 8, 64), (64, 16, 16, 16), (128, 64, 4, 128)])
+def test_long_shares(dtype, D, Hq, H, page):
+    """Enough keys that every block works through many tiles of several units."""
+    _check([3000 - 61 * i for i in range(24)], [1] * 24, Hq, H, D, page, dtype)
+
+
 @pytest.mark.parametrize("D,Hq,H", [(64, 4, 4), (128, 8, 2), (128, 3, 1), (64, 20, 1)])
 @pytest.mark.parametrize("page", [16, 64])
 def test_several_new_tokens_are_causal(D, Hq, H, page):
