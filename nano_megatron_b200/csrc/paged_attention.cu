@@ -35,7 +35,7 @@
 #include <map>
 #include <mutex>
 
-#include "paged_kv.cuh"
+#include "paged_attention.cuh"
 
 // serving.cu: shapes, types and devices of a K/V cache.
 void check_paged_cache(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_scale,
@@ -44,14 +44,18 @@ void check_paged_cache(const at::Tensor& k, const at::Tensor& v, const at::Tenso
 namespace nmb {
 namespace paged {
 
+// paged_prefill.cu
+void launch_prefill(const Params& p, int64_t D, bool int8, const at::Device& dev, cudaStream_t stream);
+
+// Requests with more query rows (new tokens x heads of a group) than this go to the prefill
+// kernel, the others to the decode kernel, which rereads the keys every 16 rows but splits them
+// over the GPU.
+constexpr int kDecodeRows = 64;
+
 constexpr int kWarps = 4;           // computing warps; one more loads
 constexpr int kThreads = (kWarps + 1) * 32;
 constexpr int kTile = 32;           // keys of a tile
 constexpr int kMinTiles = kWarps;   // tiles of a CTA's share at least: one per computing warp
-// The running max only moves when a tile exceeds it by 2^8: most tiles then skip rescaling the
-// accumulator, and P <= 256 keeps its 11 bits in f16.
-constexpr float kLazy = 8.f;
-
 // NT: 8-row tiles of query rows in a unit. The ring's length is a multiple of kWarps: tile j of a
 // CTA goes through stage j % kStages to warp j % kWarps, so one warp sees all phases of a stage's
 // barrier in order (loads land out of order, and a parity cannot tell a phase from the one
@@ -68,30 +72,6 @@ struct Cfg {
   static constexpr int kSmem = kRing + kMerge + kStats + kStages * 16 + kStages * 16 + 16;
 };
 
-struct Params {
-  const __nv_bfloat16* q;
-  int64_t q_row, q_head;
-  __nv_bfloat16* o;                 // [T, Hq, D]
-  float* lse;                       // [T, Hq] or null
-  const float *k_scale, *v_scale;
-  const int *tables, *q_starts, *kv_lens;
-  int64_t table_stride;
-  int width, num_pages, ps, page_shift;
-  int B, T, Hq, Hkv, G;
-  int max_rows;                     // requests with more query rows than this are not handled here
-  float scale_log2;
-  float* part;                      // [grid][2][rows][D] numerators of shared units
-  float2* part_ml;                  // [grid][2][rows] (M, denominator)
-  int* counters;                    // tiles finished of each shared unit; zero between calls
-  int* status;
-};
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
                                         uint32_t b1) {
   asm volatile(
@@ -99,11 +79,6 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
       "{%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 // Transposes an 8x8 matrix of f16: lane (g, t) gives [g][2t, 2t+1] and gets [2t, 2t+1][g].
@@ -854,6 +829,8 @@ at::Tensor paged_attention(at::Tensor q, at::Tensor k_pages, at::Tensor v_pages,
   p.q_head = q.stride(1);
   p.o = reinterpret_cast<__nv_bfloat16*>(o.data_ptr());
   p.lse = lse.has_value() ? lse->data_ptr<float>() : nullptr;
+  p.k_codes = static_cast<const uint8_t*>(k_pages.data_ptr());
+  p.v_codes = static_cast<const uint8_t*>(v_pages.data_ptr());
   p.k_scale = k_scale.data_ptr<float>();
   p.v_scale = v_scale.data_ptr<float>();
   p.tables = tables.data_ptr<int>();
@@ -869,12 +846,15 @@ at::Tensor paged_attention(at::Tensor q, at::Tensor k_pages, at::Tensor v_pages,
   p.Hq = static_cast<int>(Hq);
   p.Hkv = static_cast<int>(Hkv);
   p.G = static_cast<int>(Hq / Hkv);
-  p.max_rows = 1 << 30;
+  // all requests are decode's unless some may have more rows (a wrong `max_new` costs speed only)
+  const bool prefill = p.G <= 128 && max_new * p.G > kDecodeRows;
+  p.max_rows = prefill ? std::max<int>(kDecodeRows, p.G) : 1 << 30;
   p.scale_log2 = static_cast<float>(softmax_scale * 1.4426950408889634);
   p.status = status.data_ptr<int>();
   const bool i8 = k_pages.scalar_type() == at::kChar;
   // 8-row units unless some request can fill more: 16-row ones then read the cache once
   const bool wide = max_new * p.G > 8;
+  if (prefill) launch_prefill(p, D, i8, dev, stream);
   if (D == 64) {
     if (wide) i8 ? launch_decode<64, true, 2>(mk, mv, p, dev, stream) : launch_decode<64, false, 2>(mk, mv, p, dev, stream);
     else i8 ? launch_decode<64, true, 1>(mk, mv, p, dev, stream) : launch_decode<64, false, 1>(mk, mv, p, dev, stream);
