@@ -32,13 +32,15 @@ namespace paged {
 constexpr int kPfThreads = 512;
 constexpr int kPfKeys = 128;
 constexpr int kPfRows = 128;
+// Floor of the logits' factor: keeps 0 * -inf out of masked places when the softmax scale is 0.
+constexpr float kTinyScale = 1e-30f;
 // setmaxnreg shares of the four warpgroups: 2 * 184 + 104 + 40 = 4 * 128, the launch's registers
 constexpr int kRegSoftmax = 184, kRegConvert = 104, kRegIssue = 40;
 
 template <int D>
 struct PfCfg {
   static constexpr int kTile = kPfKeys * D * 2;              // one f16 tile of K, V or Q
-  static constexpr int kInfo = 4 * 8 * 8;                    // [4 tiles][8 groups of 16 keys] (ks, vs)
+  static constexpr int kInfo = 4 * 8 * 16;                   // [4 tiles][8 groups of 16 keys]
   static constexpr int kSmem = 6 * kTile + kInfo + 256;
 };
 
@@ -65,6 +67,23 @@ __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_
       : "memory");
 }
 
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)),
+        "l"(reinterpret_cast<uint64_t&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return d;
+}
+
 // kind::f16 with f16 A and B, fp32 D.
 __host__ __device__ constexpr uint32_t idesc_f16(int M, int N, bool b_mn) {
   return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | (static_cast<uint32_t>(N >> 3) << 17) |
@@ -79,7 +98,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const Params p) 
   uint8_t* sQ = smem;                                         // [2] tiles
   uint8_t* sK = sQ + 2 * C::kTile;                            // [2] stages
   uint8_t* sV = sK + 2 * C::kTile;                            // [2] stages
-  float2* s_info = reinterpret_cast<float2*>(sV + 2 * C::kTile);
+  float4* s_info = reinterpret_cast<float4*>(sV + 2 * C::kTile);  // (ks, log2 vs, 1 / vs, missing)
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_info + 4 * 8);
   uint64_t* q_full = bars;        // [2]
   uint64_t* k_full = bars + 2;    // [2]
@@ -229,7 +248,10 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const Params p) 
     constexpr int kChunks = D / 16;               // 16-code chunks of a key
     constexpr int kStep = 128 / kChunks;          // keys of one pass
     constexpr int kPass = kPfKeys / kStep;
-    const int t = tid - 256, c = t % kChunks, r0 = t / kChunks;
+    // eight lanes that store together write four chunks of two rows: all banks once
+    const int t = tid - 256;
+    const int c = D == 128 ? (t & 3) | ((t >> 1) & 4) : t & 3;
+    const int r0 = D == 128 ? ((t >> 4) << 1) | ((t >> 2) & 1) : t >> 2;
     const int* table = p.tables + b * p.table_stride;
     int pages[kPass];
     uint4 raw[2][kPass];
@@ -277,16 +299,22 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const Params p) 
       const int key = j * kPfKeys + t * 16;
       return t < 8 && key < kv ? __ldg(table + (key >> p.page_shift)) : -1;
     };
-    auto scales = [&](int page) {                 // a value scale of 0 marks a missing page
-      if (page < 0 || page >= p.num_pages) return make_float2(0.f, 0.f);
-      const int64_t u = static_cast<int64_t>(page) * p.Hkv + h;
-      return make_float2(__ldg(p.k_scale + u), __ldg(p.v_scale + u));
+    auto scales = [&](int page, int j) {
+      float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (page >= 0 && page < p.num_pages) {
+        const int64_t u = static_cast<int64_t>(page) * p.Hkv + h;
+        f.x = __ldg(p.k_scale + u);
+        f.y = __ldg(p.v_scale + u);
+      } else if (t < 8 && j * kPfKeys + t * 16 < kv) {
+        f.w = 1.f;
+      }
+      return f;
     };
     int page1 = -1;
-    float2 sc = make_float2(0.f, 0.f);
+    float4 sc = make_float4(0.f, 0.f, 0.f, 0.f);
     if (tiles > 0) {
       fetch_pages(0);
-      sc = scales(scale_page(0));
+      sc = scales(scale_page(0), 0);
       page1 = scale_page(1);
       fetch(0, 0);
       fetch(1, 0);
@@ -294,12 +322,15 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const Params p) 
     for (int j = 0; j < tiles; ++j) {
       const int st = j & 1;
       const uint32_t ph = (j >> 1) & 1;
-      const float2 sc1 = scales(page1);
+      const float4 sc1 = scales(page1, j + 1);
       page1 = scale_page(j + 2);
       if (j + 1 < tiles) fetch_pages(j + 1);
       if (!wait_warp(&k_empty[st], ph ^ 1)) break;
       convert(0, sK + st * C::kTile);
-      if (t < 8) s_info[(j & 3) * 8 + t] = sc;
+      if (t < 8) {
+        const int e = kv::exponent_of(sc.y);      // -127 where there is no page
+        s_info[(j & 3) * 8 + t] = make_float4(sc.x, static_cast<float>(e), kv::pow2i(-e), sc.w);
+      }
       sc = sc1;
       publish(&k_full[st]);
       if (j + 1 < tiles) fetch(0, j + 1);
@@ -333,8 +364,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const Params p) 
           amax = fmaxf(amax, fmaxf(fabsf(bf16_lo(w[e])), fabsf(bf16_hi(w[e]))));
       }
       const int e = min(max(kv::exponent_of(amax), -100), 126);
-      const float down = kv::pow2i(-e);
-      row_scale = kv::pow2i(e) * p.scale_log2;
+      const float down = p.scale_log2 < 0.f ? -kv::pow2i(-e) : kv::pow2i(-e);
+      row_scale = kv::pow2i(e) * fabsf(p.scale_log2);
 #pragma unroll
       for (int i = 0; i < D / 8; ++i) {
         const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
@@ -359,34 +390,33 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const Params p) 
       for (int c = 0; c < kPfKeys / 32; ++c)
         tmem_ld_32x32b_x32(tS + c * 32, *reinterpret_cast<uint32_t(*)[32]>(r + c * 32));
       tmem_wait_ld();
-      const float2* info = s_info + (j & 3) * 8;
+      const float4* info = s_info + (j & 3) * 8;
       const int key0 = j * kPfKeys;
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
       bool gap = false;
 #pragma unroll
-      for (int g = 0; g < 8; ++g) {
-        const float2 f = info[g];
-        const float a = f.x * row_scale, vb = static_cast<float>(kv::exponent_of(f.y));
-        gap = gap || f.y == 0.f;
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          r[g * 16 + e] = __float_as_uint(fmaf(__uint_as_float(r[g * 16 + e]), a, vb));
-      }
+      for (int g = 0; g < 8; ++g) gap = gap || info[g].w != 0.f;
       if (gap || key0 + kPfKeys > first_limit) {
         const int see = limit - key0;
 #pragma unroll
         for (int g = 0; g < 8; ++g) {
-          const int vis = info[g].y == 0.f ? 0 : see - g * 16;
+          const int vis = info[g].w != 0.f ? 0 : see - g * 16;
 #pragma unroll
           for (int e = 0; e < 16; ++e)
             if (e >= vis) r[g * 16 + e] = 0xff800000u;        // -inf
         }
       }
+      // The key scale is positive: a group's largest logit is that of its largest product.
+      float m_tile = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < kPfKeys; e += 4)
+      for (int g = 0; g < 8; ++g) {
+        const uint32_t* x = r + g * 16;
+        float m = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
 #pragma unroll
-        for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], __uint_as_float(r[e + k]));
-      const float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        for (int e = 2; e < 16; e += 2)
+          m = fmaxf(fmaxf(m, __uint_as_float(x[e])), __uint_as_float(x[e + 1]));
+        const float4 f = info[g];
+        m_tile = fmaxf(m_tile, fmaf(m, fmaxf(f.x * row_scale, kTinyScale), f.y));
+      }
       // (QK of this tile was issued after PV of the last one, so O is complete here.)
       if (__any_sync(0xffffffffu, m_tile > m_run + kLazy)) {
         const float m = fmaxf(m_run, m_tile);
@@ -408,17 +438,20 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const Params p) 
       const float ref = m_run == -INFINITY ? 0.f : m_run;
 #pragma unroll
       for (int g = 0; g < 8; ++g) {
-        float sum[2] = {0.f, 0.f};
+        const float4 f = info[g];
+        const float a = fmaxf(f.x * row_scale, kTinyScale), b = f.y - ref;
+        float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
         for (int e = 0; e < 16; e += 2) {
-          const float p0 = ex2(__uint_as_float(r[g * 16 + e]) - ref);
-          const float p1 = ex2(__uint_as_float(r[g * 16 + e + 1]) - ref);
-          sum[0] += p0;
-          sum[1] += p1;
-          r[g * 8 + e / 2] = f16x2(p0, p1);
+          float2 x = fma2(make_float2(__uint_as_float(r[g * 16 + e]), __uint_as_float(r[g * 16 + e + 1])),
+                          make_float2(a, a), make_float2(b, b));
+          x.x = ex2(x.x);
+          x.y = ex2(x.y);
+          sum = add2(sum, x);
+          r[g * 8 + e / 2] = f16x2(x.x, x.y);
         }
         // a missing page only adds zeros; its 2^-(-127) = 2^127 stays finite
-        l_run = fmaf(sum[0] + sum[1], kv::pow2i(-kv::exponent_of(info[g].y)), l_run);
+        l_run = fmaf(sum.x + sum.y, f.z, l_run);
       }
 #pragma unroll
       for (int c = 0; c < kPfKeys / 64; ++c) tmem_st_32x32b_x32_f(tS + c * 32, r + c * 32);
