@@ -14,8 +14,9 @@
 //   warps 8-11     : converters: cache codes from global memory (prefetched into registers one
 //                    tile ahead) to f16 tiles in shared memory, in the K-major / MN-major
 //                    128-byte-swizzled layouts that tcgen05.mma reads, two stages each of K and V;
-//   warp 12        : issues the products, alternating between the tiles: PV of the last keys, then
-//                    QK of the next, so that one tile's softmax runs under the other's products.
+//   warps 12, 13   : issue the products of tile 0 / 1: PV of the last keys, then QK of the next, so
+//                    that one tile's softmax runs under the other's products (one warp for both
+//                    was the bottleneck: about 140 cycles an instruction beside the others).
 // Codes are converted once per block and used by 256 rows; a direct 8-bit product would need
 // queries and probabilities in 8 bits.
 #include <torch/extension.h>
@@ -34,8 +35,8 @@ constexpr int kPfKeys = 128;
 constexpr int kPfRows = 128;
 // Floor of the logits' factor: keeps 0 * -inf out of masked places when the softmax scale is 0.
 constexpr float kTinyScale = 1e-30f;
-// setmaxnreg shares of the four warpgroups: 2 * 184 + 104 + 40 = 4 * 128, the launch's registers
-constexpr int kRegSoftmax = 184, kRegConvert = 104, kRegIssue = 40;
+// setmaxnreg shares of the four warpgroups: 2 * 176 + 104 + 56 = 4 * 128, the launch's registers
+constexpr int kRegSoftmax = 176, kRegConvert = 104, kRegIssue = 56;
 
 template <int D>
 struct PfCfg {
@@ -84,6 +85,43 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return d;
 }
 
+// Shared-memory matrix descriptors (128-byte swizzle, 8-row groups 1024 bytes apart) as two words:
+// the upper one is constant, and moving the start address adds to the lower one only.
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_lo(const void* p, uint32_t leading_bytes) {
+  return ((smem_u32(p) >> 4) & 0x3FFFu) | ((leading_bytes >> 4) << 16);
+}
+// A whole warp runs the issuing loop, so that addresses stay in uniform registers, and one lane
+// issues (a loop run by one lane alone spent 100 cycles a product moving them there).
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc,
+                                       uint32_t accumulate, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+      "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(kDescHi), "r"(idesc), "r"(accumulate), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t tmem_a, uint32_t b, uint32_t idesc,
+                                       uint32_t accumulate, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 b;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
+      "r"(tmem_a), "r"(b), "r"(kDescHi), "r"(idesc), "r"(accumulate), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint64_t* bar, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
+          smem_u32(bar)),
+      "r"(leader)
+      : "memory");
+}
+
 // kind::f16 with f16 A and B, fp32 D.
 __host__ __device__ constexpr uint32_t idesc_f16(int M, int N, bool b_mn) {
   return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | (static_cast<uint32_t>(N >> 3) << 17) |
@@ -107,9 +145,10 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const Params p) 
   uint64_t* v_empty = bars + 8;   // [2]
   uint64_t* s_full = bars + 10;   // [2]
   uint64_t* p_full = bars + 12;   // [2]
-  uint64_t* o_full = bars + 14;   // [1]
-  int64_t* s_find = reinterpret_cast<int64_t*>(bars + 15);    // [2] + scan in s_info
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
+  uint64_t* o_full = bars + 14;   // [2]
+  uint64_t* turn = bars + 16;     // [2] issuer r may start PV of the next tile
+  int64_t* s_find = reinterpret_cast<int64_t*>(bars + 18);    // [2] + scan in s_info
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid / 32, 0);
@@ -139,20 +178,6 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const Params p) 
       if (lane >= o) x += y;
     }
     if (lane == 31) s_scan[warp] = x;
-    if (tid == 0) {
-      for (int i = 0; i < 2; ++i) {
-        mbar_init(&q_full[i], 4);
-        mbar_init(&k_full[i], 4);
-        mbar_init(&k_empty[i], 1);
-        mbar_init(&v_full[i], 4);
-        mbar_init(&v_empty[i], 1);
-        mbar_init(&s_full[i], 1);
-        mbar_init(&p_full[i], 4);
-      }
-      mbar_init(o_full, 1);
-      *abort_flag = 0;
-      fence_mbar_init();
-    }
     __syncthreads();
     int before = x - sum, total = 0;
 #pragma unroll
@@ -186,6 +211,21 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const Params p) 
   const int tiles = (keys + kPfKeys - 1) / kPfKeys;
   const int rts = toks > tpt ? 2 : 1;
 
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 4);
+      mbar_init(&k_full[i], 4);
+      mbar_init(&k_empty[i], rts);
+      mbar_init(&v_full[i], 4);
+      mbar_init(&v_empty[i], rts);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&o_full[i], 1);
+      mbar_init(&turn[i], 1);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
   if (warp == 12) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
@@ -193,7 +233,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const Params p) 
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   // columns: S/P of tile 0, 1 at 0, 128; O of tile 0, 1 at 256, 384
   auto wait_warp = [&](uint64_t* bar, uint32_t parity) -> bool {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status, kStatusAttnTimeout, abort_flag));
@@ -201,46 +241,46 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const Params p) 
 
   if (warp >= 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegIssue));
-    if (warp == 12 && elect_one() && tiles > 0) {
-      // ---------------------------------------------------------------- product issuer
+    const int r = warp - 12;
+    if (r < rts && tiles > 0) {
+      // ------------------------------------------------- product issuer of row tile r
       constexpr uint32_t id_s = idesc_f16(kPfRows, kPfKeys, false);
       constexpr uint32_t id_o = idesc_f16(kPfRows, D, true);
-      auto wait = [&](uint64_t* bar, uint32_t parity) {
-        return mbar_wait(bar, parity, p.status, kStatusAttnTimeout, abort_flag);
-      };
-      bool ok = true;
-      auto pv = [&](int j, int r) {   // O_r += P_r V_j
-        ok = ok && wait(&p_full[r], j & 1) && wait(&v_full[j & 1], (j >> 1) & 1);
-        if (!ok) return;
-        tc_fence_after();
-        const uint32_t v = smem_u32(sV + (j & 1) * C::kTile);
-#pragma unroll
-        for (int kk = 0; kk < kPfKeys / 16; ++kk)
-          umma_f16_ts(tmem + 256 + r * 128, tmem + r * 128 + kk * 8,
-                      umma_desc_sw128(v + kk * 2048, kHalf, 1024), id_o, j > 0 || kk > 0 ? 1u : 0u);
-      };
+      const uint32_t leader = elect_one() ? 1u : 0u;
+      const uint32_t q_lo = desc_lo(sQ, 16) + r * (C::kTile >> 4);
+      const uint32_t k_lo = desc_lo(sK, 16), v_lo = desc_lo(sV, kHalf);
+      const uint32_t tS = tmem + r * 128, tO = tmem + 256 + r * 128;
+      bool ok = wait_warp(&q_full[r], 0);
       for (int j = 0; j <= tiles && ok; ++j) {
-        for (int r = 0; r < rts && ok; ++r) {
-          if (j > 0) {
-            pv(j - 1, r);
-            if (ok && r == rts - 1) umma_commit(&v_empty[(j - 1) & 1]);
-          }
-          if (!ok || j == tiles) continue;
-          ok = (j > 0 || wait(&q_full[r], 0)) && wait(&k_full[j & 1], (j >> 1) & 1);
+        if (j > 0) {                              // O += P V_{j-1}
+          const int i = j - 1;
+          ok = wait_warp(&v_full[i & 1], (i >> 1) & 1) && wait_warp(&p_full[r], i & 1) &&
+               (rts == 1 || wait_warp(&turn[r], r == 0 ? (i & 1) ^ 1 : i & 1));
           if (!ok) break;
           tc_fence_after();
-          const uint32_t q = smem_u32(sQ + r * C::kTile), k = smem_u32(sK + (j & 1) * C::kTile);
+          const uint32_t v = v_lo + (i & 1) * (C::kTile >> 4);
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = (kk >> 2) * kHalf + (kk & 3) * 32;
-            umma_f16_ss(tmem + r * 128, umma_desc_sw128(q + off, 16, 1024),
-                        umma_desc_sw128(k + off, 16, 1024), id_s, kk > 0 ? 1u : 0u);
-          }
-          umma_commit(&s_full[r]);
-          if (r == rts - 1) umma_commit(&k_empty[j & 1]);
+          for (int kk = 0; kk < kPfKeys / 16; ++kk)
+            mma_ts(tO, tS + kk * 8, v + kk * (2048 >> 4), id_o, i > 0 || kk > 0 ? 1u : 0u, leader);
+          mma_commit(j == tiles ? &o_full[r] : &v_empty[i & 1], leader);
         }
+        if (j == tiles) {
+          if (r == 0 && leader) mbar_arrive(&turn[1]);
+          break;
+        }
+        ok = wait_warp(&k_full[j & 1], (j >> 1) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t k = k_lo + (j & 1) * (C::kTile >> 4);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {     // S = Q K_j^T, over P of the last keys
+          const uint32_t off = ((kk >> 2) * kHalf + (kk & 3) * 32) >> 4;
+          mma_ss(tS, q_lo + off, k + off, id_s, kk > 0 ? 1u : 0u, leader);
+        }
+        mma_commit(&s_full[r], leader);
+        mma_commit(&k_empty[j & 1], leader);
+        if (j > 0 && leader) mbar_arrive(&turn[1 - r]);
       }
-      if (ok) umma_commit(o_full);
     }
   } else if (warp >= 8) {
     // ------------------------------------------------------------------ converters
@@ -253,24 +293,23 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const Params p) 
     const int c = D == 128 ? (t & 3) | ((t >> 1) & 4) : t & 3;
     const int r0 = D == 128 ? ((t >> 4) << 1) | ((t >> 2) & 1) : t >> 2;
     const int* table = p.tables + b * p.table_stride;
-    int pages[kPass];
     uint4 raw[2][kPass];
-    auto fetch_pages = [&](int j) {
-#pragma unroll
-      for (int i = 0; i < kPass; ++i) {
-        const int key = j * kPfKeys + i * kStep + r0;
-        const int page = key < kv ? __ldg(table + (key >> p.page_shift)) : -1;
-        pages[i] = page >= 0 && page < p.num_pages ? page : -1;
-      }
+    // Lane l < 8 of each warp holds the page of the l-th 16 keys (-1: none), two tiles ahead, and,
+    // in the first warp, their scales one tile ahead.
+    auto page_of = [&](int j) {
+      const int key = j * kPfKeys + lane * 16;
+      return lane < 8 && key < kv ? __ldg(table + (key >> p.page_shift)) : -1;
     };
-    auto fetch = [&](int which, int j) {          // stale and missing keys become code 0
-      const uint8_t* codes = which ? p.v_codes : p.k_codes;
+    auto fetch = [&](int which, int j, int page16) {   // stale and missing keys become code 0
+      const uint8_t* codes = (which ? p.v_codes : p.k_codes) + c * 16;
 #pragma unroll
       for (int i = 0; i < kPass; ++i) {
-        const int off = (j * kPfKeys + i * kStep + r0) & (p.ps - 1);
-        const int64_t row = ((static_cast<int64_t>(pages[i]) * p.Hkv + h) << p.page_shift) + off;
-        raw[which][i] = pages[i] >= 0 ? __ldg(reinterpret_cast<const uint4*>(codes + row * D) + c)
-                                      : make_uint4(0, 0, 0, 0);
+        const int in_tile = i * kStep + r0, key = j * kPfKeys + in_tile;
+        const int page = __shfl_sync(0xffffffffu, page16, in_tile >> 4);
+        const int64_t row = ((static_cast<int64_t>(page) * p.Hkv + h) << p.page_shift) + (key & (p.ps - 1));
+        raw[which][i] = key < kv && page >= 0 && page < p.num_pages
+                            ? __ldg(reinterpret_cast<const uint4*>(codes + row * D))
+                            : make_uint4(0, 0, 0, 0);
       }
     };
     auto convert = [&](int which, uint8_t* dst) {
@@ -294,37 +333,32 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const Params p) 
       __syncwarp();
       if (lane == 0) mbar_arrive(bar);
     };
-    // threads 0-7: scales of 16 keys each, pages looked up two tiles ahead and scales one
-    auto scale_page = [&](int j) {
-      const int key = j * kPfKeys + t * 16;
-      return t < 8 && key < kv ? __ldg(table + (key >> p.page_shift)) : -1;
-    };
     auto scales = [&](int page, int j) {
       float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (page >= 0 && page < p.num_pages) {
-        const int64_t u = static_cast<int64_t>(page) * p.Hkv + h;
-        f.x = __ldg(p.k_scale + u);
-        f.y = __ldg(p.v_scale + u);
-      } else if (t < 8 && j * kPfKeys + t * 16 < kv) {
-        f.w = 1.f;
+      if (t < 8) {
+        if (page >= 0 && page < p.num_pages) {
+          const int64_t u = static_cast<int64_t>(page) * p.Hkv + h;
+          f.x = __ldg(p.k_scale + u);
+          f.y = __ldg(p.v_scale + u);
+        } else if (j * kPfKeys + t * 16 < kv) {
+          f.w = 1.f;
+        }
       }
       return f;
     };
-    int page1 = -1;
     float4 sc = make_float4(0.f, 0.f, 0.f, 0.f);
+    int page1 = page_of(1);
     if (tiles > 0) {
-      fetch_pages(0);
-      sc = scales(scale_page(0), 0);
-      page1 = scale_page(1);
-      fetch(0, 0);
-      fetch(1, 0);
+      const int page0 = page_of(0);
+      sc = scales(page0, 0);
+      fetch(0, 0, page0);
+      fetch(1, 0, page0);
     }
     for (int j = 0; j < tiles; ++j) {
       const int st = j & 1;
       const uint32_t ph = (j >> 1) & 1;
       const float4 sc1 = scales(page1, j + 1);
-      page1 = scale_page(j + 2);
-      if (j + 1 < tiles) fetch_pages(j + 1);
+      const int page2 = page_of(j + 2);
       if (!wait_warp(&k_empty[st], ph ^ 1)) break;
       convert(0, sK + st * C::kTile);
       if (t < 8) {
@@ -333,11 +367,12 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const Params p) 
       }
       sc = sc1;
       publish(&k_full[st]);
-      if (j + 1 < tiles) fetch(0, j + 1);
+      if (j + 1 < tiles) fetch(0, j + 1, page1);
       if (!wait_warp(&v_empty[st], ph ^ 1)) break;
       convert(1, sV + st * C::kTile);
       publish(&v_full[st]);
-      if (j + 1 < tiles) fetch(1, j + 1);
+      if (j + 1 < tiles) fetch(1, j + 1, page1);
+      page1 = page2;
     }
   } else {
     // --------------------------------------------------------------------- softmax
@@ -461,7 +496,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const Params p) 
       if (lane == 0) mbar_arrive(&p_full[rt]);
     }
     if (rt < rts) {
-      if (tiles > 0) ok = ok && wait_warp(o_full, 0);
+      if (tiles > 0) ok = ok && wait_warp(&o_full[rt], 0);
       tc_fence_after();
       const float inv = l_run > 0.f || l_run != l_run ? 1.f / l_run : 0.f;
       const int64_t at = static_cast<int64_t>(q0 + tok) * p.Hq + h * p.G + head;
