@@ -154,81 +154,102 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
 }
 
 // ------------------------------------------------------------------------- cache write
-// One block per (touched page, kv head, K or V). The new rows are read once into registers,
-// their largest finite magnitude gives the page's scale, and the codes leave as 8-byte
-// stores; codes that were on the page before are rescaled only when the scale grows.
+// One unit is (touched page, kv head, K or V). Its new rows are read once into registers (at most
+// 16 loads of 16 bytes a lane), their largest finite magnitude gives the page's scale, and the
+// codes leave as 8-byte stores; codes that were on the page before are rescaled only when the
+// scale grows. Bound by reading the rows and writing the codes. A unit takes one warp up to 4096
+// values, so small pages need no barrier and no block of their own, two or four beyond.
 constexpr int kAppendThreads = 128;
 
 struct AppendParams {
-  const __nv_bfloat16 *x[2];
-  int64_t row_stride[2], head_stride[2];
-  uint8_t* codes[2];
-  float* scale[2];
+  const __nv_bfloat16 *k, *v;
+  int64_t k_row, k_head, v_row, v_head;
+  uint8_t *k_codes, *v_codes;
+  float *k_scale, *v_scale;
   const int4* touched;
-  int rows, num_pages, H, ps, vec;
+  int entries, rows, num_pages, H, vec;
 };
 
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, bool vec, float (&f)[8]) {
-  if (vec) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
-    f[0] = bf16_lo(v.x); f[1] = bf16_hi(v.x); f[2] = bf16_lo(v.y); f[3] = bf16_hi(v.y);
-    f[4] = bf16_lo(v.z); f[5] = bf16_hi(v.z); f[6] = bf16_lo(v.w); f[7] = bf16_hi(v.w);
-  } else {
+__device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
+  f[0] = bf16_lo(v.x); f[1] = bf16_hi(v.x); f[2] = bf16_lo(v.y); f[3] = bf16_hi(v.y);
+  f[4] = bf16_lo(v.z); f[5] = bf16_hi(v.z); f[6] = bf16_lo(v.w); f[7] = bf16_hi(v.w);
+}
+
+__device__ __forceinline__ uint4 load8(const __nv_bfloat16* p, bool vec) {
+  if (vec) return __ldg(reinterpret_cast<const uint4*>(p));
+  const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
+  uint32_t w[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = __bfloat162float(p[e]);
-  }
+  for (int e = 0; e < 4; ++e) w[e] = q[2 * e] | (static_cast<uint32_t>(q[2 * e + 1]) << 16);
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 template <bool INT8, int D, int PS>
-__global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kAppendThreads, 4) append_kernel(const AppendParams p) {
   constexpr int kCols = D / 8;                                    // 8-value chunks of a row
-  constexpr int kPer = (PS * kCols + kAppendThreads - 1) / kAppendThreads;
-  constexpr int kRowStep = kAppendThreads / kCols;
+  constexpr int kWarps = PS * D <= 4096 ? 1 : PS * D / 4096;      // of a unit
+  constexpr int kStep = kWarps * 32 / kCols;                      // rows of one pass
+  constexpr int kPer = PS / kStep;
   __shared__ float s_max[kAppendThreads / 32];
-  const int4 t = p.touched[blockIdx.x];
-  if (t.x < 0 || t.x >= p.num_pages || t.w <= 0 || t.z < 0 || t.z + t.w > PS || t.y < 0 ||
-      t.y + t.w > p.rows)
-    return;
-  const int h = blockIdx.y, which = blockIdx.z;
-  const __nv_bfloat16* x = p.x[which] + t.y * p.row_stride[which] + h * p.head_stride[which];
-  const int64_t unit = static_cast<int64_t>(t.x) * p.H + h;
-  uint8_t* codes = p.codes[which] + unit * (PS * D);
-  const int r0 = threadIdx.x / kCols, col = (threadIdx.x % kCols) * 8;
-  const float before = p.scale[which][unit];
+  const int warp = threadIdx.x / 32;
+  const int unit = blockIdx.x * (kAppendThreads / 32 / kWarps) + warp / kWarps;
+  const bool value = unit & 1;
+  const int entry = (unit >> 1) / p.H, h = (unit >> 1) - entry * p.H;
+  int4 t = make_int4(-1, 0, 0, 0);
+  if (entry < p.entries) t = __ldg(p.touched + entry);
+  const bool live = t.x >= 0 && t.x < p.num_pages && t.w > 0 && t.z >= 0 && t.z + t.w <= PS &&
+                    t.y >= 0 && t.y <= p.rows - t.w;
+  if (!live) t.w = t.z = 0;
+  const int64_t row_stride = value ? p.v_row : p.k_row;
+  const __nv_bfloat16* x = (value ? p.v : p.k) + t.y * row_stride + h * (value ? p.v_head : p.k_head);
+  const int64_t at = live ? static_cast<int64_t>(t.x) * p.H + h : 0;
+  uint8_t* codes = (value ? p.v_codes : p.k_codes) + at * (PS * D);
+  float* scale = (value ? p.v_scale : p.k_scale) + at;
+  const int lane = threadIdx.x % (kWarps * 32);
+  const int r0 = lane / kCols, col = (lane % kCols) * 8;
+  const float before = live ? *scale : 1.f;
 
-  float v[kPer][8];
+  uint4 raw[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i)
+    raw[i] = r0 + i * kStep < t.w ? load8(x + (r0 + i * kStep) * row_stride + col, p.vec)
+                                  : make_uint4(0, 0, 0, 0);
   float amax = 0.f;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    const int r = r0 + i * kRowStep;
-    if (r < t.w) {
-      load8(x + r * p.row_stride[which] + col, p.vec, v[i]);
+    float f[8];
+    unpack8(raw[i], f);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float a = fabsf(v[i][e]);
-        if (a <= 3.4e38f) amax = fmaxf(amax, a);  // infinities and NaN have no say
-      }
+    for (int e = 0; e < 8; ++e) {
+      const float a = fabsf(f[e]);
+      amax = fmaxf(amax, a <= 3.4e38f ? a : 0.f);  // infinities and NaN have no say
     }
   }
   amax = warp_max(amax);
-  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x / 32] = amax;
-  __syncthreads();
+  if constexpr (kWarps > 1) {
+    if ((threadIdx.x & 31) == 0) s_max[warp] = amax;
+    __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kAppendThreads / 32; ++i) amax = fmaxf(amax, s_max[i]);
+    for (int i = 0; i < kWarps; ++i) amax = fmaxf(amax, s_max[warp / kWarps * kWarps + i]);
+  }
+  const int old = kv::exponent_of(before);
   int e = kv::scale_exponent<INT8>(amax);
-  if (t.z > 0) e = max(e, kv::exponent_of(before));
+  if (t.z > 0) e = max(e, old);
   const float inv = kv::pow2i(-e);
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    const int r = r0 + i * kRowStep;
-    if (r < t.w)
+    const int r = r0 + i * kStep;
+    if (r < t.w) {
+      float f[8];
+      unpack8(raw[i], f);
       *reinterpret_cast<uint2*>(codes + (t.z + r) * D + col) =
-          make_uint2(kv::encode4<INT8>(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv),
-                     kv::encode4<INT8>(v[i][4] * inv, v[i][5] * inv, v[i][6] * inv, v[i][7] * inv));
+          make_uint2(kv::encode4<INT8>(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv),
+                     kv::encode4<INT8>(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
+    }
   }
-  if (t.z > 0 && e > kv::exponent_of(before)) {
-    const float f = kv::pow2i(max(kv::exponent_of(before) - e, -126));
-    for (int r = r0; r < t.z; r += kRowStep) {
+  if (t.z > 0 && e > old) {
+    const float f = kv::pow2i(max(old - e, -126));
+    for (int r = r0; r < t.z; r += kStep) {
       uint2* q = reinterpret_cast<uint2*>(codes + r * D + col);
       const uint2 c = *q;
       uint32_t w[4];
@@ -241,65 +262,81 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
                       kv::encode4<INT8>(g[2].x * f, g[2].y * f, g[3].x * f, g[3].y * f));
     }
   }
-  if (threadIdx.x == 0) p.scale[which][unit] = kv::pow2i(e);
+  if (live && lane == 0) *scale = kv::pow2i(e);
 }
 
 // -------------------------------------------------------------------------- cache read
-// out[i] = codes[slot i] * scale as bf16 (exact: 7 significant bits or fewer). 16 codes a thread.
+// out[i] = codes[slot i] * scale as bf16 (exact: 8 significant bits or fewer). Eight codes an
+// item, so that a warp's stores cover whole sectors; four items a thread in flight.
+constexpr int kReadThreads = 256;
+constexpr int kReadItems = 4;
+
 struct ReadParams {
-  const uint8_t* codes[2];
-  const float* scale[2];
-  __nv_bfloat16* out[2];
+  const uint8_t *k_codes, *v_codes;
+  const float *k_scale, *v_scale;
+  uint4 *k_out, *v_out;
   const int* slots;
-  int64_t n;          // slots * heads * (D / 16)
-  int H, D16, page_shift;
+  int64_t n;          // slots * heads * (D / 8)
+  int per_slot;       // heads * (D / 8)
+  int H, col_shift, page_shift;
   int64_t num_slots;
 };
 
 template <bool INT8>
-__global__ void __launch_bounds__(256) read_kernel(const ReadParams p) {
-  const int which = blockIdx.y;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < p.n;
-       i += static_cast<int64_t>(gridDim.x) * 256) {
-    const int c = static_cast<int>(i % p.D16);
-    const int64_t rest = i / p.D16;
-    const int h = static_cast<int>(rest % p.H);
-    const int slot = p.slots[rest / p.H];
-    uint32_t o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (slot >= 0 && slot < p.num_slots) {
-      const int64_t page = slot >> p.page_shift;
-      const int off = slot & ((1 << p.page_shift) - 1);
-      const int64_t unit = page * p.H + h;
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(p.codes[which]) +
-                            ((unit << p.page_shift) + off) * p.D16 + c);
-      const float s = __ldg(p.scale[which] + unit);
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+__global__ void __launch_bounds__(kReadThreads) read_kernel(const ReadParams p) {
+  const uint8_t* codes = blockIdx.y ? p.v_codes : p.k_codes;
+  const float* scale = blockIdx.y ? p.v_scale : p.k_scale;
+  uint4* out = blockIdx.y ? p.v_out : p.k_out;
+  const int64_t base = static_cast<int64_t>(blockIdx.x) * (kReadThreads * kReadItems);
+  const int64_t slot0 = base / p.per_slot;
+  const unsigned rem = static_cast<unsigned>(base - slot0 * p.per_slot);
+  uint2 v[kReadItems];
+  float s[kReadItems];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        uint32_t lo, hi;
-        kv::decode4<INT8>(w[k], lo, hi);
-        const float2 a = kv::f16x2_to_float2(lo), b = kv::f16x2_to_float2(hi);
-        o[2 * k] = pack_bf16x2(a.x * s, a.y * s);
-        o[2 * k + 1] = pack_bf16x2(b.x * s, b.y * s);
-      }
+  for (int k = 0; k < kReadItems; ++k) {
+    const unsigned i = k * kReadThreads + threadIdx.x;
+    v[k] = make_uint2(0, 0);
+    s[k] = 0.f;
+    if (base + i >= p.n) continue;
+    const unsigned in = (rem + i) / p.per_slot, item = rem + i - in * p.per_slot;
+    const int slot = __ldg(p.slots + slot0 + in);
+    if (slot < 0 || slot >= p.num_slots) continue;
+    const int h = item >> p.col_shift, c = item & ((1 << p.col_shift) - 1);
+    const int64_t unit = static_cast<int64_t>(slot >> p.page_shift) * p.H + h;
+    const int64_t row = (unit << p.page_shift) + (slot & ((1 << p.page_shift) - 1));
+    v[k] = __ldg(reinterpret_cast<const uint2*>(codes) + (row << p.col_shift) + c);
+    s[k] = __ldg(scale + unit);
+  }
+#pragma unroll
+  for (int k = 0; k < kReadItems; ++k) {
+    const int64_t i = base + k * kReadThreads + threadIdx.x;
+    if (i >= p.n) continue;
+    uint32_t w[4];
+    kv::decode4<INT8>(v[k].x, w[0], w[1]);
+    kv::decode4<INT8>(v[k].y, w[2], w[3]);
+    uint32_t o[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 f = kv::f16x2_to_float2(w[e]);
+      o[e] = pack_bf16x2(f.x * s[k], f.y * s[k]);
     }
-    uint4* dst = reinterpret_cast<uint4*>(p.out[which]) + i * 2;
-    dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
-    dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
+    out[i] = make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
 
 // ------------------------------------------------------------------------- logit rules
 // One block per (row, slice of the vocabulary). The block counts the row's history inside its
 // slice in shared memory (integer counts: the order of the atomics does not matter), then
-// passes once over the slice: repetition, frequency, presence, bias, allow-mask.
+// passes once over the slice, eight logits at a time: repetition, frequency, presence, mask; the
+// few biased tokens are finished after that. Bound by reading the logits and writing the scores;
+// every slice rereads the history (from L2), so slices are as long as filling the GPU allows.
 constexpr int kLogitThreads = 256;
-constexpr int kLogitSlice = 4096;
 constexpr int kMaxBias = 1024;
+constexpr int kSeen = static_cast<int>(0x80000000u);  // top bit: occurs in the prompt
 
 struct LogitParams {
   const void* logits;
-  int64_t stride;
+  int64_t stride, out_stride;
   float* out;
   const int* history;
   int64_t history_stride;
@@ -308,65 +345,91 @@ struct LogitParams {
   const int* bias_ids;
   const float* bias;
   const int* allowed;
-  int V, L, NB, words;
+  int V, L, NB, words, slice, vec;
 };
 
 __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 
+__device__ __forceinline__ void load_logits(const __nv_bfloat16* z, float (&f)[8]) {
+  unpack8(__ldg(reinterpret_cast<const uint4*>(z)), f);
+}
+__device__ __forceinline__ void load_logits(const float* z, float (&f)[8]) {
+  const float4 a = __ldg(reinterpret_cast<const float4*>(z));
+  const float4 b = __ldg(reinterpret_cast<const float4*>(z) + 1);
+  f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
+  f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kLogitThreads) logits_kernel(const LogitParams p) {
-  __shared__ int s_count[kLogitSlice];            // occurrences in the generated part
-  __shared__ uint32_t s_seen[kLogitSlice / 32];   // occurs anywhere
-  __shared__ float s_bias[kLogitSlice];
-  const int row = blockIdx.y, v0 = blockIdx.x * kLogitSlice, n = min(kLogitSlice, p.V - v0);
-  for (int i = threadIdx.x; i < kLogitSlice; i += kLogitThreads) {
-    s_count[i] = 0;
-    s_bias[i] = 0.f;
-  }
-  for (int i = threadIdx.x; i < kLogitSlice / 32; i += kLogitThreads) s_seen[i] = 0;
-  __syncthreads();
+  extern __shared__ __align__(16) int s_count[];  // [slice] occurrences; see kSeen
+  const int row = blockIdx.y, v0 = blockIdx.x * p.slice, n = min(p.slice, p.V - v0);
+  for (int i = threadIdx.x; i < p.slice / 4; i += kLogitThreads)
+    reinterpret_cast<int4*>(s_count)[i] = make_int4(0, 0, 0, 0);
   const int len = min(max(p.lens[row], 0), p.L), prompt = p.prompts[row];
+  const float rep = p.repetition ? p.repetition[row] : 1.f;
+  const float pre = p.presence ? p.presence[row] : 0.f, freq = p.frequency ? p.frequency[row] : 0.f;
+  const T* z = static_cast<const T*>(p.logits) + row * p.stride + v0;
+  float* o = p.out + row * p.out_stride + v0;
+  // the first logits are on their way while the history is counted
+  float f[8];
+  int c = threadIdx.x * 8;
+  if (p.vec && c + 8 <= n) load_logits(z + c, f);
+  __syncthreads();
   const int* hist = p.history + row * p.history_stride;
-  for (int i = threadIdx.x; i < len; i += kLogitThreads) {
-    const unsigned t = static_cast<unsigned>(hist[i]) - static_cast<unsigned>(v0);
-    if (t < static_cast<unsigned>(n)) {
-      atomicOr(&s_seen[t >> 5], 1u << (t & 31));
-      if (i >= prompt) atomicAdd(&s_count[t], 1);
-    }
-  }
-  // A token listed more than once gets the sum, in list order: its first entry adds them up.
-  for (int i = threadIdx.x; i < p.NB; i += kLogitThreads) {
-    const int* ids = p.bias_ids + static_cast<int64_t>(row) * p.NB;
-    const int id = ids[i];
-    const unsigned t = static_cast<unsigned>(id) - static_cast<unsigned>(v0);
-    if (id >= 0 && t < static_cast<unsigned>(n)) {
-      bool first = true;
-      for (int j = 0; j < i; ++j) first = first && ids[j] != id;
-      if (first) {
-        float s = 0.f;
-        for (int j = i; j < p.NB; ++j)
-          if (ids[j] == id) s += p.bias[static_cast<int64_t>(row) * p.NB + j];
-        s_bias[t] = s;
+  for (int i = threadIdx.x; i < len; i += 4 * kLogitThreads) {
+    int id[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) id[k] = i + k * kLogitThreads < len ? __ldg(hist + i + k * kLogitThreads) : -1;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const unsigned t = static_cast<unsigned>(id[k]) - static_cast<unsigned>(v0);
+      if (id[k] >= 0 && t < static_cast<unsigned>(n)) {
+        if (i + k * kLogitThreads >= prompt) atomicAdd(&s_count[t], 1);
+        else atomicOr(&s_count[t], kSeen);
       }
     }
   }
   __syncthreads();
-  const float rep = p.repetition ? p.repetition[row] : 1.f;
-  const float pre = p.presence ? p.presence[row] : 0.f, freq = p.frequency ? p.frequency[row] : 0.f;
-  const T* z = static_cast<const T*>(p.logits) + row * p.stride + v0;
-  float* o = p.out + static_cast<int64_t>(row) * p.V + v0;
-  for (int i = threadIdx.x; i < n; i += kLogitThreads) {
-    float x = to_float(z[i]);
-    if ((s_seen[i >> 5] >> (i & 31)) & 1u) x = x > 0.f ? x / rep : x * rep;
-    const int c = s_count[i];
-    if (c > 0) x = x - freq * c - pre;
-    x += s_bias[i];
-    if (p.allowed) {
-      const int v = v0 + i;
-      if (!((p.allowed[static_cast<int64_t>(row) * p.words + (v >> 5)] >> (v & 31)) & 1)) x = -INFINITY;
+  auto rule = [&](float x, int count) {
+    if (count != 0) x = x > 0.f ? x / rep : x * rep;
+    count &= ~kSeen;
+    return count > 0 ? x - freq * count - pre : x;
+  };
+  const int* allowed = p.allowed ? p.allowed + static_cast<int64_t>(row) * p.words : nullptr;
+  for (; c < n; c += kLogitThreads * 8) {
+    const unsigned bits = allowed ? static_cast<unsigned>(allowed[(v0 + c) >> 5]) >> ((v0 + c) & 31) : 255u;
+    if (p.vec && c + 8 <= n) {
+      if (c >= kLogitThreads * 8) load_logits(z + c, f);
+      const int4 n0 = reinterpret_cast<const int4*>(s_count + c)[0];
+      const int4 n1 = reinterpret_cast<const int4*>(s_count + c)[1];
+      const int cnt[8] = {n0.x, n0.y, n0.z, n0.w, n1.x, n1.y, n1.z, n1.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = (bits >> e) & 1u ? rule(f[e], cnt[e]) : -INFINITY;
+      reinterpret_cast<float4*>(o + c)[0] = make_float4(f[0], f[1], f[2], f[3]);
+      reinterpret_cast<float4*>(o + c)[1] = make_float4(f[4], f[5], f[6], f[7]);
+    } else {
+      for (int e = 0; e < 8 && c + e < n; ++e)
+        o[c + e] = (bits >> e) & 1u ? rule(to_float(z[c + e]), s_count[c + e]) : -INFINITY;
     }
-    o[i] = x;
+  }
+  if (p.NB == 0) return;
+  __syncthreads();
+  // A token listed more than once gets the sum, in list order: its first entry adds them up.
+  const int* ids = p.bias_ids + static_cast<int64_t>(row) * p.NB;
+  for (int i = threadIdx.x; i < p.NB; i += kLogitThreads) {
+    const int id = ids[i];
+    const unsigned t = static_cast<unsigned>(id) - static_cast<unsigned>(v0);
+    if (id < 0 || t >= static_cast<unsigned>(n)) continue;
+    if (allowed && !((allowed[id >> 5] >> (id & 31)) & 1)) continue;
+    bool first = true;
+    for (int j = 0; j < i; ++j) first = first && ids[j] != id;
+    if (!first) continue;
+    float s = 0.f;
+    for (int j = i; j < p.NB; ++j)
+      if (ids[j] == id) s += p.bias[static_cast<int64_t>(row) * p.NB + j];
+    o[t] += s;
   }
 }
 
@@ -444,13 +507,15 @@ std::vector<at::Tensor> plan_step(at::Tensor context, at::Tensor fresh, at::Tens
   // one allocation: [touched 4U | q_starts B+1 | kv_lens B | positions T | slots T | 2 counts]
   at::Tensor buf = at::empty({4ll * p.U + 2 * B + 1 + 2ll * p.T + 2}, context.options());
   int64_t at_ = 0;
-  auto view = [&](int64_t n) {
-    at::Tensor t = buf.narrow(0, at_, n);
-    at_ += n;
-    return t;
+  auto part = [&](at::IntArrayRef sizes) {  // a tensor over the next values (a third of a view's cost)
+    auto impl = c10::make_intrusive<c10::TensorImpl>(c10::Storage(buf.storage()), buf.key_set(), buf.dtype());
+    impl->set_storage_offset(at_);
+    impl->set_sizes_contiguous(sizes);
+    at_ += impl->numel();
+    return at::Tensor(std::move(impl));
   };
-  at::Tensor touched = view(4ll * p.U).view({p.U, 4}), q_starts = view(B + 1), kv_lens = view(B),
-             positions = view(p.T), slots = view(p.T), free_out = view(1), missing = view(1);
+  at::Tensor touched = part({p.U, 4}), q_starts = part({B + 1}), kv_lens = part({B}),
+             positions = part({p.T}), slots = part({p.T}), free_out = part({1}), missing = part({1});
   p.context = context.data_ptr<int>();
   p.fresh = fresh.data_ptr<int>();
   p.tables = tables.data_ptr<int>();
@@ -475,7 +540,7 @@ std::vector<at::Tensor> plan_step(at::Tensor context, at::Tensor fresh, at::Tens
 }
 
 template <bool INT8, int D>
-static void launch_append(const AppendParams& p, int ps, dim3 grid, cudaStream_t s) {
+static void launch_append(const AppendParams& p, int ps, unsigned grid, cudaStream_t s) {
   switch (ps) {
     case 16: append_kernel<INT8, D, 16><<<grid, kAppendThreads, 0, s>>>(p); break;
     case 32: append_kernel<INT8, D, 32><<<grid, kAppendThreads, 0, s>>>(p); break;
@@ -501,17 +566,21 @@ void append_kv(at::Tensor k_pages, at::Tensor v_pages, at::Tensor k_scale, at::T
   if (touched.size(0) == 0) return;
   AppendParams p{};
   bool vec = true;
-  for (int i = 0; i < 2; ++i) {
-    const at::Tensor& x = i ? v : k;
-    p.x[i] = reinterpret_cast<const __nv_bfloat16*>(x.data_ptr());
-    p.row_stride[i] = x.stride(0);
-    p.head_stride[i] = x.stride(1);
-    p.codes[i] = static_cast<uint8_t*>((i ? v_pages : k_pages).data_ptr());
-    p.scale[i] = (i ? v_scale : k_scale).data_ptr<float>();
-    vec = vec && reinterpret_cast<uintptr_t>(p.x[i]) % 16 == 0 && x.stride(0) % 8 == 0 &&
-          x.stride(1) % 8 == 0;
-  }
+  for (const at::Tensor* x : {&k, &v})
+    vec = vec && reinterpret_cast<uintptr_t>(x->data_ptr()) % 16 == 0 && x->stride(0) % 8 == 0 &&
+          x->stride(1) % 8 == 0;
+  p.k = reinterpret_cast<const __nv_bfloat16*>(k.data_ptr());
+  p.v = reinterpret_cast<const __nv_bfloat16*>(v.data_ptr());
+  p.k_row = k.stride(0);
+  p.k_head = k.stride(1);
+  p.v_row = v.stride(0);
+  p.v_head = v.stride(1);
+  p.k_codes = static_cast<uint8_t*>(k_pages.data_ptr());
+  p.v_codes = static_cast<uint8_t*>(v_pages.data_ptr());
+  p.k_scale = k_scale.data_ptr<float>();
+  p.v_scale = v_scale.data_ptr<float>();
   p.touched = reinterpret_cast<const int4*>(touched.data_ptr<int>());
+  p.entries = static_cast<int>(touched.size(0));
   p.rows = static_cast<int>(k.size(0));
   p.num_pages = static_cast<int>(k_pages.size(0));
   p.H = static_cast<int>(H);
@@ -519,7 +588,9 @@ void append_kv(at::Tensor k_pages, at::Tensor v_pages, at::Tensor k_scale, at::T
   const at::cuda::CUDAGuard guard(dev);
   cudaStream_t s = at::cuda::getCurrentCUDAStream();
   const int ps = static_cast<int>(k_pages.size(2));
-  const dim3 grid(touched.size(0), H, 2);
+  const int64_t units = touched.size(0) * H * 2, warps = std::max<int64_t>(1, ps * D / 4096);
+  TORCH_CHECK(units < (1ll << 31), "too many pages to write in one call");
+  const unsigned grid = static_cast<unsigned>((units * warps + 3) / 4);
   const bool i8 = k_pages.scalar_type() == at::kChar;
   if (D == 64) i8 ? launch_append<true, 64>(p, ps, grid, s) : launch_append<false, 64>(p, ps, grid, s);
   else i8 ? launch_append<true, 128>(p, ps, grid, s) : launch_append<false, 128>(p, ps, grid, s);
@@ -536,21 +607,24 @@ std::vector<at::Tensor> read_kv(at::Tensor k_pages, at::Tensor v_pages, at::Tens
   at::Tensor k = at::empty({n, H, D}, k_scale.options().dtype(at::kBFloat16)), v = at::empty_like(k);
   if (n == 0) return {k, v};
   ReadParams p{};
-  for (int i = 0; i < 2; ++i) {
-    p.codes[i] = static_cast<const uint8_t*>((i ? v_pages : k_pages).data_ptr());
-    p.scale[i] = (i ? v_scale : k_scale).data_ptr<float>();
-    p.out[i] = reinterpret_cast<__nv_bfloat16*>((i ? v : k).data_ptr());
-  }
+  p.k_codes = static_cast<const uint8_t*>(k_pages.data_ptr());
+  p.v_codes = static_cast<const uint8_t*>(v_pages.data_ptr());
+  p.k_scale = k_scale.data_ptr<float>();
+  p.v_scale = v_scale.data_ptr<float>();
+  p.k_out = reinterpret_cast<uint4*>(k.data_ptr());
+  p.v_out = reinterpret_cast<uint4*>(v.data_ptr());
   p.slots = slots.data_ptr<int>();
   p.H = static_cast<int>(H);
-  p.D16 = static_cast<int>(D / 16);
-  p.n = n * H * p.D16;
+  p.col_shift = D == 64 ? 3 : 4;
+  p.per_slot = static_cast<int>(H << p.col_shift);
+  p.n = n * p.per_slot;
   p.page_shift = page_shift_of(k_pages.size(2));
   p.num_slots = k_pages.size(0) * k_pages.size(2);
-  const dim3 grid(static_cast<unsigned>(std::min<int64_t>((p.n + 255) / 256, 148 * 16)), 2);
+  const int64_t per = kReadThreads * kReadItems;
+  const dim3 grid(static_cast<unsigned>((p.n + per - 1) / per), 2);
   cudaStream_t s = at::cuda::getCurrentCUDAStream();
-  if (k_pages.scalar_type() == at::kChar) read_kernel<true><<<grid, 256, 0, s>>>(p);
-  else read_kernel<false><<<grid, 256, 0, s>>>(p);
+  if (k_pages.scalar_type() == at::kChar) read_kernel<true><<<grid, kReadThreads, 0, s>>>(p);
+  else read_kernel<false><<<grid, kReadThreads, 0, s>>>(p);
   NMB_LAUNCHED(1);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return {k, v};
@@ -565,7 +639,7 @@ at::Tensor adjust_logits(at::Tensor logits, at::Tensor history, at::Tensor lens,
               "logits must be CUDA bf16 or fp32 [requests, vocabulary] with contiguous rows");
   const at::Device dev = logits.device();
   const int64_t B = logits.size(0), V = logits.size(1);
-  TORCH_CHECK(V < (1ll << 31) - kLogitSlice && B <= 65535, "logits are too large: ", num(B), " x ", num(V));
+  TORCH_CHECK(V < (1ll << 30) && B <= 65535, "logits are too large: ", num(B), " x ", num(V));
   TORCH_CHECK(history.device() == dev && history.scalar_type() == at::kInt && history.dim() == 2 &&
                   history.size(0) == B && (history.size(1) == 0 || history.stride(1) == 1) &&
                   history.size(1) < (1ll << 31),
@@ -605,10 +679,15 @@ at::Tensor adjust_logits(at::Tensor logits, at::Tensor history, at::Tensor lens,
     p.allowed = allowed->data_ptr<int>();
   }
   const at::cuda::CUDAGuard guard(dev);
-  at::Tensor out = at::empty({B, V}, logits.options().dtype(at::kFloat));
+  // rows padded to 32 bytes, so that every row takes wide stores
+  const int64_t pitch = (V + 7) / 8 * 8;
+  at::Tensor out = at::empty({B, pitch}, logits.options().dtype(at::kFloat));
+  if (pitch != V) out = out.narrow(1, 0, V);
   if (B == 0 || V == 0) return out;
   p.logits = logits.data_ptr();
   p.stride = logits.stride(0);
+  p.out_stride = pitch;
+  p.vec = reinterpret_cast<uintptr_t>(p.logits) % 16 == 0 && (p.stride % 8 == 0 || B == 1);
   p.out = out.data_ptr<float>();
   p.history = history.data_ptr<int>();
   p.history_stride = history.stride(0);
@@ -616,10 +695,16 @@ at::Tensor adjust_logits(at::Tensor logits, at::Tensor history, at::Tensor lens,
   p.lens = lens.data_ptr<int>();
   p.prompts = prompts.data_ptr<int>();
   p.V = static_cast<int>(V);
-  const dim3 grid((V + kLogitSlice - 1) / kLogitSlice, B);
+  // longest slice (8192: 32 KB of counts) that still gives every SM two blocks
+  int slice = 8192;
+  const int64_t want = 2ll * at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  while (slice > 512 && B * ((V + slice - 1) / slice) < want) slice /= 2;
+  p.slice = slice;
+  const dim3 grid(static_cast<unsigned>((V + slice - 1) / slice), static_cast<unsigned>(B));
+  const size_t smem = slice * sizeof(int);
   cudaStream_t s = at::cuda::getCurrentCUDAStream();
-  if (logits.scalar_type() == at::kFloat) logits_kernel<float><<<grid, kLogitThreads, 0, s>>>(p);
-  else logits_kernel<__nv_bfloat16><<<grid, kLogitThreads, 0, s>>>(p);
+  if (logits.scalar_type() == at::kFloat) logits_kernel<float><<<grid, kLogitThreads, smem, s>>>(p);
+  else logits_kernel<__nv_bfloat16><<<grid, kLogitThreads, smem, s>>>(p);
   NMB_LAUNCHED(1);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return out;
