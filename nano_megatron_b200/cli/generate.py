@@ -7,14 +7,23 @@ import json
 from collections.abc import Sequence
 from pathlib import Path
 
-from nano_megatron_b200.inference import GenerationResult, generate_from_artifact
+from nano_megatron_b200.inference import (
+    GenerationResult,
+    LogitRules,
+    generate_batch_from_artifact,
+    generate_from_artifact,
+)
 
 
 def parser() -> argparse.ArgumentParser:
     p = argparse.ArgumentParser(description=__doc__)
     p.add_argument("--model", type=Path, required=True,
                    help="artifact directory written by nano-megatron-export")
-    p.add_argument("--prompt", required=True, help="text to continue")
+    what = p.add_mutually_exclusive_group(required=True)
+    what.add_argument("--prompt", help="text to continue")
+    what.add_argument("--prompts-file", type=Path,
+                      help="continue every line of this file, served as one batch over an 8-bit "
+                           "paged K/V cache; prints one result per line, in order")
     p.add_argument("--device", default="auto",
                    help="'auto' uses CUDA when it is available; or cpu, cuda, cuda:N")
     p.add_argument("--dtype", choices=("auto", "float32", "bfloat16", "float16"),
@@ -34,6 +43,16 @@ def parser() -> argparse.ArgumentParser:
     p.add_argument("--kv-cache", action=argparse.BooleanOptionalAction, default=True,
                    help="reuse cached keys/values between decode steps (on by default; "
                         "--no-kv-cache recomputes the whole prefix every step)")
+    b = p.add_argument_group("batched generation (--prompts-file)")
+    b.add_argument("--max-batch", type=int, default=64, help="prompts served at a time")
+    b.add_argument("--cache-dtype", choices=("e4m3", "int8"), default="e4m3",
+                   help="8-bit format of the K/V cache")
+    b.add_argument("--repetition-penalty", type=float, default=1.0,
+                   help="divide positive scores of tokens seen before by this (1 = off)")
+    b.add_argument("--presence-penalty", type=float, default=0.0,
+                   help="subtract this from tokens that were generated before")
+    b.add_argument("--frequency-penalty", type=float, default=0.0,
+                   help="subtract this once per earlier generation of a token")
     p.add_argument("--json", action="store_true",
                    help="print the whole result (prompt, completion, token ids, stop reason) "
                         "as one JSON object instead of the text")
@@ -52,6 +71,18 @@ def run_generate(model: Path, prompt: str, *, device: str = "auto", dtype: str =
 
 def main(argv: Sequence[str] | None = None) -> None:
     a = parser().parse_args(argv)
+    if a.prompts_file is not None:
+        prompts = a.prompts_file.read_text(encoding="utf-8").splitlines()
+        for r in generate_batch_from_artifact(
+                a.model, prompts, device=a.device, dtype=a.dtype,
+                max_new_tokens=a.max_new_tokens, temperature=a.temperature, top_p=a.top_p,
+                top_k=a.top_k, seed=a.seed, add_bos=a.add_bos, max_batch=a.max_batch,
+                cache_dtype=a.cache_dtype,
+                rules=LogitRules(repetition=a.repetition_penalty, presence=a.presence_penalty,
+                                 frequency=a.frequency_penalty)):
+            print(json.dumps(r.to_dict(), ensure_ascii=False, sort_keys=True) if a.json
+                  else r.text.replace("\n", " "))
+        return
     r = run_generate(a.model, a.prompt, device=a.device, dtype=a.dtype,
                      max_new_tokens=a.max_new_tokens, temperature=a.temperature, top_p=a.top_p,
                      top_k=a.top_k, seed=a.seed, add_bos=a.add_bos, kv_cache=a.kv_cache)

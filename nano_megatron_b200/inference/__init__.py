@@ -1,4 +1,4 @@
-"""Checkpoint export to single-device artifacts and KV-cached generation."""
+"""Checkpoint export to single-device artifacts, KV-cached and batched generation."""
 
 from .artifact import (
     ARTIFACT_NAME,
@@ -8,6 +8,7 @@ from .artifact import (
     export_checkpoint,
     load_inference_artifact,
 )
+from .batch import BatchDecoder, LogitRules, generate_batch, generate_batch_from_artifact
 from .generation import (
     GenerationResult,
     KVCacheDecoder,
@@ -17,7 +18,8 @@ from .generation import (
     sample_next_token,
 )
 
-__all__ = ["ARTIFACT_NAME", "ARTIFACT_VERSION", "GenerationResult", "InferenceArtifact",
-           "InferenceArtifactError", "KVCacheDecoder", "export_checkpoint",
+__all__ = ["ARTIFACT_NAME", "ARTIFACT_VERSION", "BatchDecoder", "GenerationResult",
+           "InferenceArtifact", "InferenceArtifactError", "KVCacheDecoder", "LogitRules",
+           "export_checkpoint", "generate_batch", "generate_batch_from_artifact",
            "generate_from_artifact", "generate_text", "load_inference_artifact",
            "load_model_for_generation", "sample_next_token"]

@@ -127,11 +127,30 @@ def sample_next_token(logits: torch.Tensor, *, temperature: float, top_p: float,
     return int(torch.multinomial(probs, 1, generator=generator))
 
 
+def fused_layer_weights(model) -> list[dict]:
+    """Per layer, the weights in the form the decoders use: norms, ``[q; k; v]`` and
+    ``[gate; up]`` stacked, output and down projections, and their biases (None without)."""
+    bias = bool(getattr(model.config, "bias", False))
+    layers = []
+    for layer in model.layers:
+        at, mlp = layer.attention, layer.mlp
+        qkv = [m.linear for m in (at.q_proj, at.k_proj, at.v_proj)]
+        gu = [mlp.gate_proj.linear, mlp.up_proj.linear]
+        layers.append(dict(
+            n1=layer.input_norm.weight, n2=layer.post_attention_norm.weight,
+            wqkv=torch.cat([m.weight for m in qkv]).contiguous(),
+            bqkv=torch.cat([m.bias for m in qkv]) if bias else None,
+            wo=at.out_proj.linear.weight, bo=at.out_proj.linear.bias if bias else None,
+            wgu=torch.cat([m.weight for m in gu]).contiguous(),
+            bgu=torch.cat([m.bias for m in gu]) if bias else None,
+            wd=mlp.down_proj.linear.weight, bd=mlp.down_proj.linear.bias if bias else None))
+    return layers
+
+
 class KVCacheDecoder:
     """Incremental decoder over a single-device ``GPTModel``'s weights."""
 
     def __init__(self, model, max_len: int) -> None:
-        cfg = model.config
         self.model = model
         a0 = model.layers[0].attention
         self.nh, self.nkv, self.d = a0.num_heads, a0.num_kv_heads, a0.head_dim
@@ -141,25 +160,9 @@ class KVCacheDecoder:
         dev = model.embedding.weight.device
         dt = model.embedding.weight.dtype
         self.inv_freq = model.rope_inv_freq.to(dev)
-        self.bias = bool(getattr(cfg, "bias", False))
-        self.layers = []
-        for layer in model.layers:
-            at, mlp = layer.attention, layer.mlp
-            wqkv = torch.cat([at.q_proj.linear.weight, at.k_proj.linear.weight,
-                              at.v_proj.linear.weight]).contiguous()
-            bqkv = torch.cat([at.q_proj.linear.bias, at.k_proj.linear.bias,
-                              at.v_proj.linear.bias]) if self.bias else None
-            wgu = torch.cat([mlp.gate_proj.linear.weight, mlp.up_proj.linear.weight]).contiguous()
-            bgu = torch.cat([mlp.gate_proj.linear.bias, mlp.up_proj.linear.bias]) \
-                if self.bias else None
-            self.layers.append(dict(
-                n1=layer.input_norm.weight, n2=layer.post_attention_norm.weight,
-                wqkv=wqkv, bqkv=bqkv, wo=at.out_proj.linear.weight,
-                bo=at.out_proj.linear.bias if self.bias else None, wgu=wgu, bgu=bgu,
-                wd=mlp.down_proj.linear.weight,
-                bd=mlp.down_proj.linear.bias if self.bias else None,
-                k=torch.empty(self.max_len, self.nkv, self.d, device=dev, dtype=dt),
-                v=torch.empty(self.max_len, self.nkv, self.d, device=dev, dtype=dt)))
+        self.layers = [dict(w, k=torch.empty(self.max_len, self.nkv, self.d, device=dev, dtype=dt),
+                            v=torch.empty(self.max_len, self.nkv, self.d, device=dev, dtype=dt))
+                       for w in fused_layer_weights(model)]
         self.length = 0
 
     @staticmethod
