@@ -174,30 +174,36 @@ __global__ void __launch_bounds__(Cfg<D, NT, NW>::kThreads, Cfg<D, NT, NW>::kCta
     return;
   }
 
-  // Rows past the last request's (padding) are zero.
-  {
-    const int used = min(max(__ldg(p.q_starts + p.B), 0), p.T);
-    if (used < p.T) {
-      const int64_t n = static_cast<int64_t>(p.T - used) * p.Hq * (D / 8);
-      uint4* o4 = reinterpret_cast<uint4*>(p.o) + static_cast<int64_t>(used) * p.Hq * (D / 8);
-      for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + tid; i < n;
-           i += static_cast<int64_t>(gridDim.x) * kThreads) {
-        o4[i] = make_uint4(0, 0, 0, 0);
-        if (p.lse != nullptr && i % (D / 8) == 0)
-          p.lse[static_cast<int64_t>(used) * p.Hq + i / (D / 8)] = -INFINITY;
-      }
+  // Rows past the last request's (padding) are zero; written at the end.
+  const int used = min(max(__ldg(p.q_starts + p.B), 0), p.T);
+  auto zero_padding = [&] {
+    constexpr int threads = NW * 32;
+    if (used >= p.T || tid >= threads) return;
+    const int64_t n = static_cast<int64_t>(p.T - used) * p.Hq * (D / 8);
+    uint4* o4 = reinterpret_cast<uint4*>(p.o) + static_cast<int64_t>(used) * p.Hq * (D / 8);
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * threads + tid; i < n;
+         i += static_cast<int64_t>(gridDim.x) * threads) {
+      o4[i] = make_uint4(0, 0, 0, 0);
+      if (p.lse != nullptr && i % (D / 8) == 0)
+        p.lse[static_cast<int64_t>(used) * p.Hq + i / (D / 8)] = -INFINITY;
     }
-  }
+  };
 
   // ---- this CTA's share of the tiles
+  // CTA c has tiles [c * share + min(c, extra), ...): equal to one tile, 32-bit arithmetic.
   Cursor<NT> cur;
-  int total, ctas;
+  int ctas, share, extra;
   {
     int64_t* s_scan = reinterpret_cast<int64_t*>(s_merge);  // free until the first merge
+    int* s_found = reinterpret_cast<int*>(s_scan + 16);
     const int per = (p.B + kThreads - 1) / kThreads;
     const int b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
     int64_t sum = 0;
-    for (int b = b0; b < b1; ++b) sum += load_request<NT>(p, b).total(p.Hkv);
+    Request r{0, 0, 0, 0, 1};
+    for (int b = b0; b < b1; ++b) {
+      r = load_request<NT>(p, b);
+      sum += r.total(p.Hkv);
+    }
     int64_t x = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -205,14 +211,12 @@ __global__ void __launch_bounds__(Cfg<D, NT, NW>::kThreads, Cfg<D, NT, NW>::kCta
       if (lane >= o) x += y;
     }
     if (lane == 31) s_scan[warp] = x;
-    if (tid == 0) {
-      for (int i = 0; i < S; ++i) {
-        mbar_init(&full[i], 1);
-        mbar_init(&empty[i], 1);
-      }
-      s_flag[0] = 0;
+    if (tid < S) {
+      mbar_init(&full[tid], 1);
+      mbar_init(&empty[tid], 1);
       fence_mbar_init();
     }
+    if (tid == 0) s_flag[0] = 0;
     __syncthreads();
     int64_t before = x - sum, all = 0;
 #pragma unroll
@@ -224,26 +228,36 @@ __global__ void __launch_bounds__(Cfg<D, NT, NW>::kThreads, Cfg<D, NT, NW>::kCta
       if (tid == 0) record_status(p.status, kStatusAttnTimeout);
       return;
     }
-    total = static_cast<int>(all);
+    const int total = static_cast<int>(all);
     ctas = min(static_cast<int>(gridDim.x), (total + C::kMinTiles - 1) / C::kMinTiles);
-    if (static_cast<int>(blockIdx.x) >= ctas) return;
-    cur.g = static_cast<int>(static_cast<int64_t>(blockIdx.x) * total / ctas);
-    cur.end = static_cast<int>((blockIdx.x + 1ll) * total / ctas);
+    const int cta = blockIdx.x;
+    if (cta >= ctas) {
+      zero_padding();
+      return;
+    }
+    share = total / ctas;
+    extra = total - share * ctas;
+    cur.g = cta * share + min(cta, extra);
+    cur.end = cur.g + share + (cta < extra ? 1 : 0);
     if (before <= cur.g && cur.g < before + sum) {
-      int b = b0;
-      int64_t base = before;
-      for (;; ++b) {
-        const int64_t t = load_request<NT>(p, b).total(p.Hkv);
-        if (cur.g < base + t || b + 1 >= b1) break;
-        base += t;
+      int b = b0, base = static_cast<int>(before);
+      if (per > 1) r = load_request<NT>(p, b);
+      while (b + 1 < b1 && cur.g >= base + static_cast<int>(r.total(p.Hkv))) {
+        base += static_cast<int>(r.total(p.Hkv));
+        r = load_request<NT>(p, ++b);
       }
-      s_scan[16] = b;
-      s_scan[17] = base;
+      s_found[0] = b;
+      s_found[1] = base;
+      s_found[2] = r.q0;
+      s_found[3] = r.nq;
+      s_found[4] = r.kv;
+      s_found[5] = r.blocks;
+      s_found[6] = r.tiles;
     }
     __syncthreads();
-    cur.b = static_cast<int>(s_scan[16]);
-    cur.base = static_cast<int>(s_scan[17]);
-    cur.r = load_request<NT>(p, cur.b);
+    cur.b = s_found[0];
+    cur.base = s_found[1];
+    cur.r = Request{s_found[2], s_found[3], s_found[4], s_found[5], s_found[6]};
     cur.set();
     __syncthreads();  // the merge area is free again
   }
@@ -302,11 +316,10 @@ __global__ void __launch_bounds__(Cfg<D, NT, NW>::kThreads, Cfg<D, NT, NW>::kCta
         ok = wait_warp(&empty[stage], ((j / S) & 1) ^ 1);
         if (!ok) break;
         if (lane == i) {
-          s_info[stage] = info;
+          // The copies first: they need no scales. (Bytes may land before they are announced; the
+          // phase cannot end before the arrival.)
           uint8_t* dst = ring + stage * C::kStageBytes;
           const uint32_t bytes = (ok0 ? 2u * box * D : 0u) + (two && ok1 ? 2u * box * D : 0u);
-          if (bytes) mbar_arrive_expect_tx(&full[stage], bytes);
-          else mbar_arrive(&full[stage]);
           if (ok0) {
             const int y = static_cast<int>(u0 << p.page_shift) + t.off;
             tma_load_2d(dst, &tmK, &full[stage], 0, y);
@@ -317,6 +330,9 @@ __global__ void __launch_bounds__(Cfg<D, NT, NW>::kThreads, Cfg<D, NT, NW>::kCta
             tma_load_2d(dst + 16 * D, &tmK, &full[stage], 0, y);
             tma_load_2d(dst + kTile * D + 16 * D, &tmV, &full[stage], 0, y);
           }
+          s_info[stage] = info;
+          if (bytes) mbar_arrive_expect_tx(&full[stage], bytes);
+          else mbar_arrive(&full[stage]);
         }
         __syncwarp();
       }
@@ -620,11 +636,11 @@ __global__ void __launch_bounds__(Cfg<D, NT, NW>::kThreads, Cfg<D, NT, NW>::kCta
     if (whole) continue;
 
     // ---- a unit shared with other CTAs: the last to finish adds the parts up in CTA order
-    __threadfence();
     sync_all();
     const int rpt = (p.G + kRows - 1) / kRows;
     if (tid == 0) {
       int* counter = p.counters + (static_cast<int64_t>(h) * p.T + cur.r.q0) * rpt + rb;
+      __threadfence();              // the barrier and this fence publish the whole CTA's part
       const int before = atomicAdd(counter, cur.n);
       const bool last = before + cur.n == cur.r.tiles;
       if (last) *counter = 0;
@@ -634,72 +650,79 @@ __global__ void __launch_bounds__(Cfg<D, NT, NW>::kThreads, Cfg<D, NT, NW>::kCta
     sync_all();
     if (s_flag[1]) {
       const int u0 = cur.base + cur.unit * cur.r.tiles, u1 = u0 + cur.r.tiles;
-      auto owner = [&](int tile) { return static_cast<int>(((tile + 1ll) * ctas - 1) / total); };
+      auto owner = [&](int tile) {
+        const int longer = extra * (share + 1);
+        return tile < longer ? tile / (share + 1) : extra + (tile - longer) / share;
+      };
       const int c0 = owner(u0), n = owner(u1 - 1) - c0 + 1;
       // only the first of them can have had another unit before this one
-      const int first = c0 * 2 + (static_cast<int64_t>(c0) * total / ctas >= u0 ? 0 : 1);
+      const int first = c0 * 2 + (c0 * share + min(c0, extra) >= u0 ? 0 : 1);
       auto slot_of = [&](int i) { return i == 0 ? first : (c0 + i) * 2; };
       // A warp, or several that share the parts, per row. Lanes hold the weights of 32 parts at a
       // time and 4 columns each (D = 64: the halves of the warp take every other part).
       constexpr int kHalves = 128 / D;
       const int col = (lane & (D / 4 - 1)) * 4, odd = lane / (D / 4);
-      const int at_once = min(rows, NW), share = NW / at_once;   // rows, warps of a row
+      const int at_once = min(rows, NW), helpers = NW / at_once;   // rows, warps of a row
       for (int row0 = 0; row0 < rows; row0 += at_once) {
         const int row = row0 + warp % at_once, mine = warp / at_once;
-        const bool live = row < rows && mine < share;
-        const int from = live ? n * mine / share : 0, to = live ? n * (mine + 1) / share : 0;
-        float m = -INFINITY;
-        if (live)
-          for (int i = lane; i < n; i += 32) m = fmaxf(m, __ldcg(&p.part_ml[slot_of(i) * kRows + row]).x);
-        m = warp_max(m);
-        const float ref = m == -INFINITY ? 0.f : m;
-        float l = 0.f;
+        const bool live = row < rows && mine < helpers;
+        const int from = live ? n * mine / helpers : 0, to = live ? n * (mine + 1) / helpers : 0;
+        float m = -INFINITY, l = 0.f;
         float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int i0 = from; i0 < to; i0 += 32) {
-          float w = 0.f;
-          if (i0 + lane < to) {
-            const float2 ml = __ldcg(&p.part_ml[slot_of(i0 + lane) * kRows + row]);
-            w = ex2(ml.x - ref);
-            l = fmaf(ml.y, w, l);
-          }
+        constexpr int kBatch = 16 / kHalves;      // parts of a lane in flight
 #pragma unroll 1
-          for (int k0 = 0; k0 < 32 && i0 + k0 < to; k0 += 16) {
-            float4 y[16 / kHalves];
+        for (int i0 = from; i0 < to; i0 += 16) {
+          float4 y[kBatch];
 #pragma unroll
-            for (int k = 0; k < 16 / kHalves; ++k) {
-              const int i = min(i0 + k0 + k * kHalves + odd, to - 1);
-              y[k] = __ldcg(reinterpret_cast<const float4*>(
-                  p.part + (static_cast<int64_t>(slot_of(i)) * kRows + row) * D + col));
-            }
+          for (int k = 0; k < kBatch; ++k) {
+            const int i = min(i0 + k * kHalves + odd, to - 1);
+            y[k] = __ldcg(reinterpret_cast<const float4*>(
+                p.part + (static_cast<int64_t>(slot_of(i)) * kRows + row) * D + col));
+          }
+          float2 ml = make_float2(-INFINITY, 0.f);
+          if (lane < 16 && i0 + lane < to) ml = __ldcg(&p.part_ml[slot_of(i0 + lane) * kRows + row]);
+          const float top = fmaxf(m, warp_max(ml.x)), ref = top == -INFINITY ? 0.f : top;
+          const float w = ex2(ml.x - ref), down = ex2(m - ref);   // 0 past the last part
+          m = top;
+          l = fmaf(l, down, warp_sum(ml.y * w));
+          x.x *= down; x.y *= down; x.z *= down; x.w *= down;
 #pragma unroll
-            for (int k = 0; k < 16 / kHalves; ++k) {
-              const float f = __shfl_sync(0xffffffffu, w, k0 + k * kHalves + odd);
-              const bool in = i0 + k0 + k * kHalves + odd < to;
-              x.x = in ? fmaf(y[k].x, f, x.x) : x.x;
-              x.y = in ? fmaf(y[k].y, f, x.y) : x.y;
-              x.z = in ? fmaf(y[k].z, f, x.z) : x.z;
-              x.w = in ? fmaf(y[k].w, f, x.w) : x.w;
-            }
+          for (int k = 0; k < kBatch; ++k) {
+            const float f = __shfl_sync(0xffffffffu, w, k * kHalves + odd);
+            const bool in = i0 + k * kHalves + odd < to;
+            x.x = in ? fmaf(y[k].x, f, x.x) : x.x;
+            x.y = in ? fmaf(y[k].y, f, x.y) : x.y;
+            x.z = in ? fmaf(y[k].z, f, x.z) : x.z;
+            x.w = in ? fmaf(y[k].w, f, x.w) : x.w;
           }
         }
-        l = warp_sum(l);
         if constexpr (kHalves == 2) {
           x.x += __shfl_xor_sync(0xffffffffu, x.x, 16);
           x.y += __shfl_xor_sync(0xffffffffu, x.y, 16);
           x.z += __shfl_xor_sync(0xffffffffu, x.z, 16);
           x.w += __shfl_xor_sync(0xffffffffu, x.w, 16);
         }
-        if (share > 1) {            // the row's first warp adds the others' sums, in order
+        if (helpers > 1) {          // the row's first warp adds the others' sums, in order
           float* s_sum = reinterpret_cast<float*>(s_merge);
           if (odd == 0) *reinterpret_cast<float4*>(s_sum + warp * D + col) = x;
-          if (lane == 0) s_stat[warp].x = l;
+          if (lane == 0) s_stat[warp] = make_float2(m, l);
           sync_all();
-          if (mine == 0)
-            for (int k = 1; k < share; ++k) {
+          if (mine == 0) {
+            float top = m;
+            for (int k = 1; k < helpers; ++k) top = fmaxf(top, s_stat[warp + k * at_once].x);
+            const float ref = top == -INFINITY ? 0.f : top, down = ex2(m - ref);
+            m = top;
+            l *= down;
+            x.x *= down; x.y *= down; x.z *= down; x.w *= down;
+            for (int k = 1; k < helpers; ++k) {
+              const float2 st = s_stat[warp + k * at_once];
+              const float f = ex2(st.x - ref);
               const float4 y = *reinterpret_cast<const float4*>(s_sum + (warp + k * at_once) * D + col);
-              x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
-              l += s_stat[warp + k * at_once].x;
+              x.x = fmaf(y.x, f, x.x); x.y = fmaf(y.y, f, x.y);
+              x.z = fmaf(y.z, f, x.z); x.w = fmaf(y.w, f, x.w);
+              l = fmaf(st.y, f, l);
             }
+          }
           sync_all();
         }
         if (!live || mine != 0) continue;
@@ -713,6 +736,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, NW>::kThreads, Cfg<D, NT, NW>::kCta
       }
     }
   }
+  zero_padding();
 }
 
 template <int D, bool INT8, int NT, int NW>
