@@ -518,6 +518,45 @@ __global__ void __launch_bounds__(Cfg<D, NT, NW>::kThreads, Cfg<D, NT, NW>::kCta
         }
       }
 
+      // NaN among the values of keys that some rows see and others do not: 0 * NaN would reach
+      // the others. The rows that see one get NaN here, and the code becomes 0 in this stage.
+      if (!INT8 && masked && cur.r.nq > 1) {
+        constexpr int kWords = D / 32;            // this lane's columns: D / 8 codes of each key
+        uint32_t* mine = reinterpret_cast<uint32_t*>(const_cast<uint8_t*>(sv));
+        auto word_at = [&](int r) {
+          return (chunk_at<D>(r, D == 128 ? (g8 >> 1) | ((g8 & 1) << 2) : g8 >> 1) +
+                  (D == 128 ? 0 : (g8 & 1) * 8)) / 4;
+        };
+        uint32_t any = 0;
+#pragma unroll 1
+        for (int r = 0; r < kTile; ++r)
+#pragma unroll
+          for (int w = 0; w < kWords; ++w) {
+            const uint32_t bad = kv::nan_bytes(mine[word_at(r) + w]);
+            any |= bad;
+            if (bad == 0) continue;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int c = 0; c < 2; ++c)
+                if (key0 + r < limit[nt][c] && (r < 16 ? f.z : f.w) != 0.f)
+#pragma unroll
+                  for (int e = 0; e < 4; ++e)
+                    if ((bad >> (8 * e)) & 0x80u)
+                      acc[nt][2 * w + e / 2][(e & 1) * 2 + c] = __int_as_float(0x7fffffff);
+          }
+        if (__any_sync(0xffffffffu, any != 0)) {
+#pragma unroll 1
+          for (int r = 0; r < kTile && t4 == 0; ++r)
+            for (int w = 0; w < kWords; ++w) {
+              uint32_t& x = mine[word_at(r) + w];
+              x &= ~((kv::nan_bytes(x) >> 7) * 255u);
+            }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the stage is TMA's next
+          __syncwarp();
+        }
+      }
+
       // O^T += V^T P^T
       const bool tail = key0 + kTile > cur.r.kv || f.z == 0.f || f.w == 0.f;
 #pragma unroll

@@ -81,6 +81,11 @@ __device__ __forceinline__ void decode4(uint32_t v, uint32_t& lo, uint32_t& hi) 
   }
 }
 
+// 0x80 in each byte of `v` that is the NaN of e4m3 (0x7F or 0xFF).
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t v) {
+  return ((v & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+}
+
 __device__ __forceinline__ float2 f16x2_to_float2(uint32_t v) {
   return __half22float2(*reinterpret_cast<__half2*>(&v));
 }

@@ -150,6 +150,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const Params p) 
   int64_t* s_find = reinterpret_cast<int64_t*>(bars + 18);    // [2] + scan in s_info
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* s_nan = abort_flag + 1;           // NaN among values that only some rows see
 
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid / 32, 0);
   if (smem_u32(smem) & 1023u) {
@@ -224,6 +225,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const Params p) 
       mbar_init(&turn[i], 1);
     }
     *abort_flag = 0;
+    *s_nan = 0;
     fence_mbar_init();
   }
   if (warp == 12) {
@@ -369,6 +371,22 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const Params p) 
       publish(&k_full[st]);
       if (j + 1 < tiles) fetch(0, j + 1, page1);
       if (!wait_warp(&v_empty[st], ph ^ 1)) break;
+      if (!INT8 && (j + 1) * kPfKeys > kv - n + tok0 + 1) {
+        // keys that some rows see and others do not: 0 * NaN would reach the others, so NaN
+        // counts as 0 in the product and is put in at the end
+        uint32_t bad = 0;
+#pragma unroll
+        for (int i = 0; i < kPass; ++i) {
+          uint32_t* x = reinterpret_cast<uint32_t*>(&raw[1][i]);
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t m = kv::nan_bytes(x[w]);
+            bad |= m;
+            x[w] &= ~((m >> 7) * 255u);
+          }
+        }
+        if (bad) *s_nan = 1;
+      }
       convert(1, sV + st * C::kTile);
       publish(&v_full[st]);
       if (j + 1 < tiles) fetch(1, j + 1, page1);
@@ -501,6 +519,20 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const Params p) 
       const float inv = l_run > 0.f || l_run != l_run ? 1.f / l_run : 0.f;
       const int64_t at = static_cast<int64_t>(q0 + tok) * p.Hq + h * p.G + head;
       __nv_bfloat16* dst = p.o + at * D;
+      uint32_t nan_cols[D / 32] = {};
+      if (!INT8 && tiles > 0 && *s_nan) {         // which columns of the keys this row sees
+        const int* table = p.tables + b * p.table_stride;
+        for (int key = max(0, kv - n + tok0 + 1) / kPfKeys * kPfKeys; key < min(limit, kv); ++key) {
+          const int page = __ldg(table + (key >> p.page_shift));
+          if (page < 0 || page >= p.num_pages) continue;
+          const uint8_t* x = p.v_codes + (((static_cast<int64_t>(page) * p.Hkv + h) << p.page_shift) +
+                                          (key & (p.ps - 1))) * D;
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c)
+            for (int e = 0; e < 32; ++e)
+              nan_cols[c] |= static_cast<uint32_t>((x[c * 32 + e] & 0x7F) == 0x7F) << e;
+        }
+      }
       if (ok) {
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
@@ -509,6 +541,10 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const Params p) 
             tmem_ld_32x32b_x32(tO + c * 32, o);
             tmem_wait_ld();
           }
+          if (!INT8 && nan_cols[c] != 0)
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if ((nan_cols[c] >> e) & 1u) o[e] = 0x7fffffffu;
           if (live) {
             // a row that saw nothing has 0 in O or, without any tile, nothing there
 #pragma unroll

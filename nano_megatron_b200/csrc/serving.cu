@@ -331,6 +331,7 @@ __global__ void __launch_bounds__(kReadThreads) read_kernel(const ReadParams p) 
 // few biased tokens are finished after that. Bound by reading the logits and writing the scores;
 // every slice rereads the history (from L2), so slices are as long as filling the GPU allows.
 constexpr int kLogitThreads = 256;
+constexpr int kLogitSlice = 8192;   // the longest: 32 KB of counts, four loads a thread
 constexpr int kMaxBias = 1024;
 constexpr int kSeen = static_cast<int>(0x80000000u);  // top bit: occurs in the prompt
 
@@ -351,15 +352,24 @@ struct LogitParams {
 __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-__device__ __forceinline__ void load_logits(const __nv_bfloat16* z, float (&f)[8]) {
-  unpack8(__ldg(reinterpret_cast<const uint4*>(z)), f);
-}
-__device__ __forceinline__ void load_logits(const float* z, float (&f)[8]) {
-  const float4 a = __ldg(reinterpret_cast<const float4*>(z));
-  const float4 b = __ldg(reinterpret_cast<const float4*>(z) + 1);
-  f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-  f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-}
+// Eight logits in flight, as loaded.
+template <typename T> struct Raw8;
+template <> struct Raw8<__nv_bfloat16> {
+  uint4 v;
+  __device__ void load(const __nv_bfloat16* z) { v = __ldg(reinterpret_cast<const uint4*>(z)); }
+  __device__ void get(float (&f)[8]) const { unpack8(v, f); }
+};
+template <> struct Raw8<float> {
+  float4 a, b;
+  __device__ void load(const float* z) {
+    a = __ldg(reinterpret_cast<const float4*>(z));
+    b = __ldg(reinterpret_cast<const float4*>(z) + 1);
+  }
+  __device__ void get(float (&f)[8]) const {
+    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
+    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+  }
+};
 
 template <typename T>
 __global__ void __launch_bounds__(kLogitThreads) logits_kernel(const LogitParams p) {
@@ -372,10 +382,14 @@ __global__ void __launch_bounds__(kLogitThreads) logits_kernel(const LogitParams
   const float pre = p.presence ? p.presence[row] : 0.f, freq = p.frequency ? p.frequency[row] : 0.f;
   const T* z = static_cast<const T*>(p.logits) + row * p.stride + v0;
   float* o = p.out + row * p.out_stride + v0;
-  // the first logits are on their way while the history is counted
-  float f[8];
-  int c = threadIdx.x * 8;
-  if (p.vec && c + 8 <= n) load_logits(z + c, f);
+  // all of the slice's logits are on their way while the history is counted
+  constexpr int kPasses = kLogitSlice / (kLogitThreads * 8);
+  Raw8<T> raw[kPasses];
+#pragma unroll
+  for (int i = 0; i < kPasses; ++i) {
+    const int c = (i * kLogitThreads + threadIdx.x) * 8;
+    if (p.vec && c + 8 <= n) raw[i].load(z + c);
+  }
   __syncthreads();
   const int* hist = p.history + row * p.history_stride;
   for (int i = threadIdx.x; i < len; i += 4 * kLogitThreads) {
@@ -398,15 +412,23 @@ __global__ void __launch_bounds__(kLogitThreads) logits_kernel(const LogitParams
     return count > 0 ? x - freq * count - pre : x;
   };
   const int* allowed = p.allowed ? p.allowed + static_cast<int64_t>(row) * p.words : nullptr;
-  for (; c < n; c += kLogitThreads * 8) {
+#pragma unroll
+  for (int i = 0; i < kPasses; ++i) {
+    const int c = (i * kLogitThreads + threadIdx.x) * 8;
+    if (c >= n) break;
     const unsigned bits = allowed ? static_cast<unsigned>(allowed[(v0 + c) >> 5]) >> ((v0 + c) & 31) : 255u;
     if (p.vec && c + 8 <= n) {
-      if (c >= kLogitThreads * 8) load_logits(z + c, f);
+      float f[8];
+      raw[i].get(f);
       const int4 n0 = reinterpret_cast<const int4*>(s_count + c)[0];
       const int4 n1 = reinterpret_cast<const int4*>(s_count + c)[1];
       const int cnt[8] = {n0.x, n0.y, n0.z, n0.w, n1.x, n1.y, n1.z, n1.w};
+      if ((n0.x | n0.y | n0.z | n0.w | n1.x | n1.y | n1.z | n1.w) != 0) {  // few tokens occurred
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = (bits >> e) & 1u ? rule(f[e], cnt[e]) : -INFINITY;
+        for (int e = 0; e < 8; ++e) f[e] = rule(f[e], cnt[e]);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = (bits >> e) & 1u ? f[e] : -INFINITY;
       reinterpret_cast<float4*>(o + c)[0] = make_float4(f[0], f[1], f[2], f[3]);
       reinterpret_cast<float4*>(o + c)[1] = make_float4(f[4], f[5], f[6], f[7]);
     } else {
@@ -695,8 +717,8 @@ at::Tensor adjust_logits(at::Tensor logits, at::Tensor history, at::Tensor lens,
   p.lens = lens.data_ptr<int>();
   p.prompts = prompts.data_ptr<int>();
   p.V = static_cast<int>(V);
-  // longest slice (8192: 32 KB of counts) that still gives every SM two blocks
-  int slice = 8192;
+  // longest slice that still gives every SM two blocks
+  int slice = kLogitSlice;
   const int64_t want = 2ll * at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
   while (slice > 512 && B * ((V + slice - 1) / slice) < want) slice /= 2;
   p.slice = slice;

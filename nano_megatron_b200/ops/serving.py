@@ -208,7 +208,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, tables: torch.Tensor,
     positions; a row sees its own position and those before it. ``heads`` is a multiple of the
     cache's kv heads (grouped queries). ``max_new`` is an upper bound of the rows of one request.
     Rows past ``q_starts[B]`` and rows that see no key give 0; positions on a missing page
-    (table entry -1) are not seen. ``lse`` (fp32 [tokens, heads]) receives the base-2
+    (table entry -1) are not seen. NaN in a position reaches the rows that see it and no others. ``lse`` (fp32 [tokens, heads]) receives the base-2
     log-sum-exp of the scaled scores, -inf for rows that see nothing.
     """
     D = cache.k_pages.shape[3]
@@ -246,7 +246,11 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, tables: torch.Tensor,
         s = s.masked_fill(~seen, -math.inf)
         z = torch.logsumexp(s, -1)
         p = torch.where(z[..., None] == -math.inf, 0.0, torch.exp(s - z[..., None]))
-        out[r0:r1] = (p @ dense(cache.v_pages, cache.v_scale)).transpose(0, 1).to(q.dtype)
+        v = dense(cache.v_pages, cache.v_scale)
+        bad = v.isnan()                       # reaches the rows that see it and no others
+        o = p @ torch.where(bad, 0.0, v)
+        o = torch.where(seen.to(cd) @ bad.to(cd) > 0, math.nan, o)
+        out[r0:r1] = o.transpose(0, 1).to(q.dtype)
         if lse is not None:
             lse[r0:r1] = (z / math.log(2.0)).transpose(0, 1).float()
     return out

@@ -346,6 +346,30 @@ def test_large_scores():
     _check([300], [200], 8, 2, 128, 64, E4M3, level=30.0)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Hq,n", [(2, 4), (6, 5), (2, 20), (4, 150), (2, 300)])
+def test_nan_reaches_only_the_rows_that_see_it(D, Hq, n):
+    """NaN keys and values among the new tokens: earlier rows are as without them; later rows are
+    NaN (a NaN key) or NaN in the value's column."""
+    ctx = 37
+    cache, tables = _filled([ctx + n], 2, D, 16, E4M3)
+    q = torch.randn(n, 2 * Hq, D, device=DEV).bfloat16()
+    args = (tables, ints([0, n]), ints([ctx + n]))
+    clean = serving.paged_attention(q, cache, *args, max_new=n)
+    first = n // 2                       # row whose position holds the NaN value of head 0
+    pos = ctx + first
+    page, off = int(tables[0, pos // 16]), pos % 16
+    cache.v_pages.view(torch.uint8)[page, 0, off, 5] = 0xFF
+    later = ctx + n - 1                  # the last position's key of head 1
+    cache.k_pages.view(torch.uint8)[int(tables[0, later // 16]), 1, later % 16, 3] = 0x7F
+    got = serving.paged_attention(q, cache, *args, max_new=n)
+    assert torch.equal(got[:first], clean[:first])
+    assert bool(got[first:, :Hq, 5].isnan().all())
+    others = [c for c in range(D) if c != 5]
+    assert torch.equal(got[:, :Hq][..., others], clean[:, :Hq][..., others])
+    assert torch.equal(got[:-1, Hq:], clean[:-1, Hq:]) and bool(got[-1, Hq:].isnan().all())
+
+
 def test_row_offsets_past_the_keys_see_nothing():
     """kv_lens smaller than the rows (a caller's error): the first rows see no key and give 0."""
     cache, tables = _filled([20], 1, 64, 16, E4M3)
