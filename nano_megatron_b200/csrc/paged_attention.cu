@@ -26,7 +26,9 @@ void launch_prefill(const Params& p, int64_t D, bool int8, const at::Device& dev
 
 // Requests with more query rows (new tokens x heads of a group) than this go to the prefill
 // kernel, the others to the decode kernel, which rereads the keys every 16 rows but splits them
-// over the GPU.
+// over the GPU. At 68 rows, 8 kv heads of 128: 32 requests of 256 / 4096 cached tokens take 79 / 308 us
+// in the decode kernel and 37 / 199 in the other, 2 requests 33 / 42 and 21 / 91 us; at 256 rows
+// the decode kernel only wins for the 2 long ones (73 for 102 us).
 constexpr int kDecodeRows = 64;
 
 static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {

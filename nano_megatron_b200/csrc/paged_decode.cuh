@@ -48,23 +48,26 @@ struct Scratch {
 Scratch scratch_for(const at::Device& dev, cudaStream_t stream, int64_t part, int64_t counters);
 
 constexpr int kTile = 32;           // keys of a tile
-// NT: 8-row tiles of query rows in a unit. NW: computing warps of a CTA. Twelve in one CTA an SM
-// where there are few units (each is then cut into few parts, which the last CTA joins), four in
-// three or four CTAs otherwise (one CTA's unit ends are hidden by the others).
-// The ring's length is a multiple of NW: tile j of a CTA goes through stage j % kStages to warp
-// j % NW, so one warp sees all phases of a stage's barrier in order (loads land out of order, and
-// a parity cannot tell a phase from the one before the last).
-template <int D, int NT, int NW>
+// Computing warps of a CTA; one more loads. (Twelve in one CTA an SM, for few units, gave 21.0 for
+// 21.3 us at one request of 32k tokens and lost up to a quarter at 18 requests: 33.7 for 25 us at
+// 2048 tokens. One CTA's unit ends are not hidden by others then.)
+constexpr int kWarps = 4;
+constexpr int kThreads = (kWarps + 1) * 32;
+constexpr int kMinTiles = kWarps;   // tiles of a CTA's share at least (8: 11.4 for 10.0 us at 1 x 512)
+
+// NT: 8-row tiles of query rows in a unit. The ring's length is a multiple of kWarps: tile j of a
+// CTA goes through stage j % kStages to warp j % kWarps, so one warp sees all phases of a stage's
+// barrier in order (loads land out of order, and a parity cannot tell a phase from the one
+// before the last).
+template <int D, int NT>
 struct Cfg {
-  static constexpr int kThreads = (NW + 1) * 32;            // and a loading warp
-  static constexpr int kCtasPerSm = NW == 12 ? 1 : NT == 2 ? 2 : D == 128 ? 3 : 4;
-  static constexpr int kStages = NW == 12 ? 24 : NT == 1 ? 8 : D == 128 ? 12 : 16;
-  static_assert(kStages % NW == 0, "a stage belongs to one warp");
-  static constexpr int kMinTiles = NW == 12 ? 16 : 4;       // of a CTA's share
+  static constexpr int kCtasPerSm = NT == 2 ? 2 : D == 128 ? 3 : 4;
+  static constexpr int kStages = NT == 1 ? 8 : D == 128 ? 12 : 16;
+  static_assert(kStages % kWarps == 0, "a stage belongs to one warp");
   static constexpr int kStageBytes = 2 * kTile * D;
   static constexpr int kRing = kStages * kStageBytes;
-  static constexpr int kMerge = NW * 8 * 64 * 4;            // 8 rows by 64 columns at a time
-  static constexpr int kStats = (NW + 1) * 8 * NT * 8;
+  static constexpr int kMerge = kWarps * 8 * 64 * 4;        // 8 rows by 64 columns at a time
+  static constexpr int kStats = (kWarps + 1) * 8 * NT * 8;
   static constexpr int kSmem = kRing + kMerge + kStats + kStages * 16 + kStages * 16 + 16;
 };
 
@@ -149,12 +152,11 @@ __device__ __forceinline__ int merge_at(int row, int u) {
   return row * 16 + (u ^ (D == 128 ? t : (t & 1) | ((t >> 1) << 2)));
 }
 
-template <int D, bool INT8, int NT, int NW>
-__global__ void __launch_bounds__(Cfg<D, NT, NW>::kThreads, Cfg<D, NT, NW>::kCtasPerSm)
+template <int D, bool INT8, int NT>
+__global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtasPerSm)
     decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                   const Params p) {
-  using C = Cfg<D, NT, NW>;
-  constexpr int kThreads = C::kThreads;
+  using C = Cfg<D, NT>;
   constexpr int S = C::kStages;
   constexpr int kSteps = D / 16;
   constexpr int kRows = 8 * NT;
@@ -162,7 +164,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, NW>::kThreads, Cfg<D, NT, NW>::kCta
   uint8_t* ring = smem;
   float4* s_merge = reinterpret_cast<float4*>(smem + C::kRing);
   float2* s_stat = reinterpret_cast<float2*>(smem + C::kRing + C::kMerge);   // [warp][row] (M, l)
-  float2* s_tot = s_stat + NW * kRows;                                   // [row]
+  float2* s_tot = s_stat + kWarps * kRows;                                   // [row]
   float4* s_info = reinterpret_cast<float4*>(s_tot + kRows);                 // [S] scales
   uint64_t* full = reinterpret_cast<uint64_t*>(s_info + S);
   uint64_t* empty = full + S;
@@ -177,7 +179,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, NW>::kThreads, Cfg<D, NT, NW>::kCta
   // Rows past the last request's (padding) are zero; written at the end.
   const int used = min(max(__ldg(p.q_starts + p.B), 0), p.T);
   auto zero_padding = [&] {
-    constexpr int threads = NW * 32;
+    constexpr int threads = kWarps * 32;
     if (used >= p.T || tid >= threads) return;
     const int64_t n = static_cast<int64_t>(p.T - used) * p.Hq * (D / 8);
     uint4* o4 = reinterpret_cast<uint4*>(p.o) + static_cast<int64_t>(used) * p.Hq * (D / 8);
@@ -220,7 +222,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, NW>::kThreads, Cfg<D, NT, NW>::kCta
     __syncthreads();
     int64_t before = x - sum, all = 0;
 #pragma unroll
-    for (int i = 0; i <= NW; ++i) {
+    for (int i = 0; i <= kWarps; ++i) {
       if (i < warp) before += s_scan[i];
       all += s_scan[i];
     }
@@ -229,7 +231,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, NW>::kThreads, Cfg<D, NT, NW>::kCta
       return;
     }
     const int total = static_cast<int>(all);
-    ctas = min(static_cast<int>(gridDim.x), (total + C::kMinTiles - 1) / C::kMinTiles);
+    ctas = min(static_cast<int>(gridDim.x), (total + kMinTiles - 1) / kMinTiles);
     const int cta = blockIdx.x;
     if (cta >= ctas) {
       zero_padding();
@@ -268,7 +270,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, NW>::kThreads, Cfg<D, NT, NW>::kCta
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status, kStatusAttnTimeout, s_flag));
   };
 
-  if (warp == NW) {
+  if (warp == kWarps) {
     // ---------------------------------------------------------------- loading warp
     const bool two = p.ps < kTile;
     const int box = two ? p.ps : kTile;
@@ -349,7 +351,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, NW>::kThreads, Cfg<D, NT, NW>::kCta
   const int g8 = lane >> 2, t4 = lane & 3;
   auto sync_all = [] {
     __syncwarp();
-    asm volatile("bar.sync 1, %0;" ::"n"(NW * 32) : "memory");
+    asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory");
   };
   int j0 = 0;                       // tiles of this CTA before the run
   bool ok = true;
@@ -416,7 +418,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, NW>::kThreads, Cfg<D, NT, NW>::kCta
     const int free_keys = cur.r.kv - cur.r.nq + rb * kRows / p.G + 1;  // keys that every row sees
 
 #pragma unroll 1
-    for (int i = (warp + NW - j0 % NW) % NW; i < cur.n; i += NW) {
+    for (int i = (warp - j0) & (kWarps - 1); i < cur.n; i += kWarps) {
       const int stage = (j0 + i) % S;
       if (ok) ok = wait_warp(&full[stage], ((j0 + i) / S) & 1);
       if (!ok) break;
@@ -617,10 +619,10 @@ __global__ void __launch_bounds__(Cfg<D, NT, NW>::kThreads, Cfg<D, NT, NW>::kCta
         const int row = nt * 8 + 2 * t4 + c;
         float m = -INFINITY, l = 0.f;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) m = fmaxf(m, s_stat[w * kRows + row].x);
+        for (int w = 0; w < kWarps; ++w) m = fmaxf(m, s_stat[w * kRows + row].x);
         const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) {
+        for (int w = 0; w < kWarps; ++w) {
           const float2 st = s_stat[w * kRows + row];
           l = fmaf(st.y, ex2(st.x - ref), l);
         }
@@ -649,11 +651,11 @@ __global__ void __launch_bounds__(Cfg<D, NT, NW>::kThreads, Cfg<D, NT, NW>::kCta
       }
       sync_all();
       const int in = min(8, rows - nt * 8);
-      for (int u = tid; u < in * 16; u += NW * 32) {
+      for (int u = tid; u < in * 16; u += kWarps * 32) {
         const int r8 = u / 16, q = part_cols * 16 + u % 16, row = nt * 8 + r8;
         float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < NW; ++w) {
+        for (int w = 0; w < kWarps; ++w) {
           const float4 y = s_merge[w * 8 * 16 + merge_at<D>(r8, u % 16)];
           x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
         }
@@ -701,7 +703,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, NW>::kThreads, Cfg<D, NT, NW>::kCta
       // time and 4 columns each (D = 64: the halves of the warp take every other part).
       constexpr int kHalves = 128 / D;
       const int col = (lane & (D / 4 - 1)) * 4, odd = lane / (D / 4);
-      const int at_once = min(rows, NW), helpers = NW / at_once;   // rows, warps of a row
+      const int at_once = min(rows, kWarps), helpers = kWarps / at_once;   // rows, warps of a row
       for (int row0 = 0; row0 < rows; row0 += at_once) {
         const int row = row0 + warp % at_once, mine = warp / at_once;
         const bool live = row < rows && mine < helpers;
@@ -778,13 +780,13 @@ __global__ void __launch_bounds__(Cfg<D, NT, NW>::kThreads, Cfg<D, NT, NW>::kCta
   zero_padding();
 }
 
-template <int D, bool INT8, int NT, int NW>
+template <int D, bool INT8, int NT>
 static void launch_decode_as(const CUtensorMap& mk, const CUtensorMap& mv, Params& p,
                           const at::Device& dev, cudaStream_t stream) {
-  using C = Cfg<D, NT, NW>;
+  using C = Cfg<D, NT>;
   static std::once_flag once[64];
   std::call_once(once[dev.index() & 63], [] {
-    C10_CUDA_CHECK(cudaFuncSetAttribute(decode_kernel<D, INT8, NT, NW>,
+    C10_CUDA_CHECK(cudaFuncSetAttribute(decode_kernel<D, INT8, NT>,
                                         cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
   });
   const int grid = at::cuda::getCurrentDeviceProperties()->multiProcessorCount * C::kCtasPerSm;
@@ -794,27 +796,21 @@ static void launch_decode_as(const CUtensorMap& mk, const CUtensorMap& mv, Param
   p.part = scratch.part.data_ptr<float>();
   p.part_ml = reinterpret_cast<float2*>(p.part + slots * D);
   p.counters = scratch.counters.data_ptr<int>();
-  decode_kernel<D, INT8, NT, NW><<<grid, C::kThreads, C::kSmem, stream>>>(mk, mv, p);
+  decode_kernel<D, INT8, NT><<<grid, kThreads, C::kSmem, stream>>>(mk, mv, p);
   NMB_LAUNCHED(1);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
-// 8-row units unless some request can fill more: 16-row ones then read the cache once. Twelve
-// warps a CTA where there cannot be more units than SMs (decode 1 x 32k: 21 us with four).
+// 8-row units unless some request can fill more: 16-row ones then read the cache once.
 template <int D>
 static void launch_decode_for(const CUtensorMap& mk, const CUtensorMap& mv, Params& p, int64_t max_new,
                               bool int8, const at::Device& dev, cudaStream_t stream) {
-  const int64_t rows = max_new * p.G;
-  const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-  if (rows > 8)
-    int8 ? launch_decode_as<D, true, 2, 4>(mk, mv, p, dev, stream)
-         : launch_decode_as<D, false, 2, 4>(mk, mv, p, dev, stream);
-  else if (static_cast<int64_t>(p.B) * p.Hkv <= sms)
-    int8 ? launch_decode_as<D, true, 1, 12>(mk, mv, p, dev, stream)
-         : launch_decode_as<D, false, 1, 12>(mk, mv, p, dev, stream);
+  if (max_new * p.G > 8)
+    int8 ? launch_decode_as<D, true, 2>(mk, mv, p, dev, stream)
+         : launch_decode_as<D, false, 2>(mk, mv, p, dev, stream);
   else
-    int8 ? launch_decode_as<D, true, 1, 4>(mk, mv, p, dev, stream)
-         : launch_decode_as<D, false, 1, 4>(mk, mv, p, dev, stream);
+    int8 ? launch_decode_as<D, true, 1>(mk, mv, p, dev, stream)
+         : launch_decode_as<D, false, 1>(mk, mv, p, dev, stream);
 }
 
 }  // namespace paged
