@@ -152,7 +152,8 @@ __device__ __forceinline__ int merge_at(int row, int u) {
   return row * 16 + (u ^ (D == 128 ? t : (t & 1) | ((t >> 1) << 2)));
 }
 
-template <int D, bool INT8, int NT>
+// SEVERAL: requests may have several new tokens, so that a key can be hidden from some rows only.
+template <int D, bool INT8, int NT, bool SEVERAL>
 __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtasPerSm)
     decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                   const Params p) {
@@ -522,7 +523,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtasPerSm)
 
       // NaN among the values of keys that some rows see and others do not: 0 * NaN would reach
       // the others. The rows that see one get NaN here, and the code becomes 0 in this stage.
-      if (!INT8 && masked && cur.r.nq > 1) {
+      if (SEVERAL && !INT8 && masked && cur.r.nq > 1) {
         constexpr int kWords = D / 32;            // this lane's columns: D / 8 codes of each key
         uint32_t* mine = reinterpret_cast<uint32_t*>(const_cast<uint8_t*>(sv));
         auto word_at = [&](int r) {
@@ -780,13 +781,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtasPerSm)
   zero_padding();
 }
 
-template <int D, bool INT8, int NT>
+template <int D, bool INT8, int NT, bool SEVERAL>
 static void launch_decode_as(const CUtensorMap& mk, const CUtensorMap& mv, Params& p,
                           const at::Device& dev, cudaStream_t stream) {
   using C = Cfg<D, NT>;
   static std::once_flag once[64];
   std::call_once(once[dev.index() & 63], [] {
-    C10_CUDA_CHECK(cudaFuncSetAttribute(decode_kernel<D, INT8, NT>,
+    C10_CUDA_CHECK(cudaFuncSetAttribute(decode_kernel<D, INT8, NT, SEVERAL>,
                                         cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
   });
   const int grid = at::cuda::getCurrentDeviceProperties()->multiProcessorCount * C::kCtasPerSm;
@@ -796,7 +797,7 @@ static void launch_decode_as(const CUtensorMap& mk, const CUtensorMap& mv, Param
   p.part = scratch.part.data_ptr<float>();
   p.part_ml = reinterpret_cast<float2*>(p.part + slots * D);
   p.counters = scratch.counters.data_ptr<int>();
-  decode_kernel<D, INT8, NT><<<grid, kThreads, C::kSmem, stream>>>(mk, mv, p);
+  decode_kernel<D, INT8, NT, SEVERAL><<<grid, kThreads, C::kSmem, stream>>>(mk, mv, p);
   NMB_LAUNCHED(1);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
@@ -806,11 +807,14 @@ template <int D>
 static void launch_decode_for(const CUtensorMap& mk, const CUtensorMap& mv, Params& p, int64_t max_new,
                               bool int8, const at::Device& dev, cudaStream_t stream) {
   if (max_new * p.G > 8)
-    int8 ? launch_decode_as<D, true, 2>(mk, mv, p, dev, stream)
-         : launch_decode_as<D, false, 2>(mk, mv, p, dev, stream);
+    int8 ? launch_decode_as<D, true, 2, true>(mk, mv, p, dev, stream)
+         : launch_decode_as<D, false, 2, true>(mk, mv, p, dev, stream);
+  else if (int8)
+    launch_decode_as<D, true, 1, true>(mk, mv, p, dev, stream);
+  else if (max_new > 1)
+    launch_decode_as<D, false, 1, true>(mk, mv, p, dev, stream);
   else
-    int8 ? launch_decode_as<D, true, 1>(mk, mv, p, dev, stream)
-         : launch_decode_as<D, false, 1>(mk, mv, p, dev, stream);
+    launch_decode_as<D, false, 1, false>(mk, mv, p, dev, stream);
 }
 
 }  // namespace paged
