@@ -392,12 +392,12 @@ __global__ void __launch_bounds__(kLogitThreads) logits_kernel(const LogitParams
   }
   __syncthreads();
   const int* hist = p.history + row * p.history_stride;
-  for (int i = threadIdx.x; i < len; i += 4 * kLogitThreads) {
-    int id[4];
+  for (int i = threadIdx.x; i < len; i += 8 * kLogitThreads) {
+    int id[8]; 
 #pragma unroll
-    for (int k = 0; k < 4; ++k) id[k] = i + k * kLogitThreads < len ? __ldg(hist + i + k * kLogitThreads) : -1;
+    for (int k = 0; k < 8; ++k) id[k] = i + k * kLogitThreads < len ? __ldg(hist + i + k * kLogitThreads) : -1;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < 8; ++k) {
       const unsigned t = static_cast<unsigned>(id[k]) - static_cast<unsigned>(v0);
       if (id[k] >= 0 && t < static_cast<unsigned>(n)) {
         if (i + k * kLogitThreads >= prompt) atomicAdd(&s_count[t], 1);
@@ -406,8 +406,10 @@ __global__ void __launch_bounds__(kLogitThreads) logits_kernel(const LogitParams
     }
   }
   __syncthreads();
+  // one reciprocal a row: x * (1 / rep) is within 1.5 ulp of x / rep and an eighth of its work
+  const float inv = 1.f / rep;
   auto rule = [&](float x, int count) {
-    if (count != 0) x = x > 0.f ? x / rep : x * rep;
+    if (count != 0) x *= x > 0.f ? inv : rep;
     count &= ~kSeen;
     return count > 0 ? x - freq * count - pre : x;
   };
@@ -438,20 +440,26 @@ __global__ void __launch_bounds__(kLogitThreads) logits_kernel(const LogitParams
   }
   if (p.NB == 0) return;
   __syncthreads();
-  // A token listed more than once gets the sum, in list order: its first entry adds them up.
+  // A warp per entry, its lanes looking for the same token in the list. A token listed more than
+  // once gets the sum, in list order: its first entry adds them up.
   const int* ids = p.bias_ids + static_cast<int64_t>(row) * p.NB;
-  for (int i = threadIdx.x; i < p.NB; i += kLogitThreads) {
-    const int id = ids[i];
+  const float* values = p.bias + static_cast<int64_t>(row) * p.NB;
+  const int lane = threadIdx.x & 31;
+  for (int i = threadIdx.x / 32; i < p.NB; i += kLogitThreads / 32) {
+    const int id = __ldg(ids + i);
     const unsigned t = static_cast<unsigned>(id) - static_cast<unsigned>(v0);
     if (id < 0 || t >= static_cast<unsigned>(n)) continue;
     if (allowed && !((allowed[id >> 5] >> (id & 31)) & 1)) continue;
-    bool first = true;
-    for (int j = 0; j < i; ++j) first = first && ids[j] != id;
-    if (!first) continue;
     float s = 0.f;
-    for (int j = i; j < p.NB; ++j)
-      if (ids[j] == id) s += p.bias[static_cast<int64_t>(row) * p.NB + j];
-    o[t] += s;
+    bool first = true;
+    for (int j0 = 0; j0 < p.NB && first; j0 += 32) {
+      const bool same = j0 + lane < p.NB && __ldg(ids + j0 + lane) == id;
+      const float x = same ? __ldg(values + j0 + lane) : 0.f;
+      unsigned hits = __ballot_sync(0xffffffffu, same);
+      first = hits == 0 || j0 + __ffs(hits) - 1 >= i;
+      for (; hits && first; hits &= hits - 1) s += __shfl_sync(0xffffffffu, x, __ffs(hits) - 1);
+    }
+    if (first && lane == 0) o[t] += s;
   }
 }
 
