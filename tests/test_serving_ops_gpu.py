@@ -380,7 +380,49 @@ def test_row_offsets_past_the_keys_see_nothing():
     assert o[10:].abs().amax((1, 2)).min() > 0
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_rows_at_odd_addresses(D):
+    """Rows that start at odd elements: the scalar loads of the cache write, a copied query."""
+    T, H = 23, 2
+    wide = torch.randn(T, 3 * H * D + 1, device=DEV).bfloat16()
+    q, k, v = (wide[:, 1 + i * H * D:1 + (i + 1) * H * D].view(T, H, D) for i in range(3))
+    assert k.data_ptr() % 16 and k.stride(0) % 8
+    touched = ints([[1, 0, 0, 16], [0, 16, 0, 7]])
+    odd, even = _cache(2, H, D, 16, E4M3), _cache(2, H, D, 16, E4M3)
+    serving.append_kv(odd, k, v, touched)
+    serving.append_kv(even, k.contiguous(), v.contiguous(), touched)
+    for a, b in zip(odd, even):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    args = (odd, ints([[1, 0]]), ints([0, T]), ints([T]))
+    assert torch.equal(serving.paged_attention(q, *args, max_new=T),
+                       serving.paged_attention(q.contiguous(), *args, max_new=T))
+
+
+def test_cache_beyond_4_gib():
+    """Pages whose byte offsets pass 32 bits: write, read back, decode, prompt."""
+    H, D, page, pages = 8, 128, 64, 70000                # 4.6 GB of codes each
+    cache = serving.PagedKV.create(pages, H, D, page_size=page)
+    small = serving.PagedKV.create(4, H, D, page_size=page)
+    far = [pages - 1, 65536, pages - 2, 3]
+    x = torch.randn(230, 2, H, D, device=DEV).bfloat16()
+    rows = [(0, 64), (64, 64), (128, 64), (192, 38)]
+    for c, ids in ((cache, far), (small, [0, 1, 2, 3])):
+        serving.append_kv(c, x[:, 0], x[:, 1], ints([[p, r, 0, n] for p, (r, n) in zip(ids, rows)]))
+    slots = [[p * page + i for p, (_, n) in zip(ids, rows) for i in range(n)]
+             for ids in (far, [0, 1, 2, 3])]
+    for a, b in zip(serving.read_kv(cache, ints(slots[0])), serving.read_kv(small, ints(slots[1]))):
+        assert torch.equal(a, b)
+    for n in (1, 200):
+        q = torch.randn(n, 4 * H, D, device=DEV).bfloat16()
+        a, b = (serving.paged_attention(q, c, ints([ids]), ints([0, n]), ints([230]), max_new=n)
+                for c, ids in ((cache, far), (small, [0, 1, 2, 3])))
+        assert torch.equal(a, b) and bool(a.isfinite().all())
+
+
 def test_empty_calls():
+    p = serving.plan_step(ints([]), ints([]), torch.zeros(0, 1, dtype=torch.int32, device=DEV),
+                          ints([0]), ints([1]), page_size=16, num_tokens=3)
+    assert p.q_starts.tolist() == [0] and p.slots.tolist() == [-1] * 3 and p.free_count.item() == 1
     cache, tables = _filled([20], 1, 64, 16, E4M3)
     q = torch.empty(0, 2, 64, device=DEV, dtype=torch.bfloat16)
     assert serving.paged_attention(q, cache, tables, ints([0, 0]), ints([20]), max_new=0).shape == (0, 2, 64)
