@@ -194,9 +194,16 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtasPerSm)
   };
 
   // ---- this CTA's share of the tiles
-  // CTA c has tiles [c * share + min(c, extra), ...): equal to one tile, 32-bit arithmetic.
+  // Groups of `per` CTAs have `span` tiles each, the i-th of a group from i * share + min(i, extra)
+  // on: equal to one tile. One group is all there is, but for a single request, whose units have
+  // equal lengths: a group a unit then, so that no CTA merges two
+  // (decode 1 x 32k: 22.7 -> 20.3 us).
   Cursor<NT> cur;
-  int ctas, share, extra;
+  int span, per_group, share, extra;
+  auto start_of = [&](int c) {
+    const int group = c / per_group, i = c - group * per_group;
+    return group * span + i * share + min(i, extra);
+  };
   {
     int64_t* s_scan = reinterpret_cast<int64_t*>(s_merge);  // free until the first merge
     int* s_found = reinterpret_cast<int*>(s_scan + 16);
@@ -233,16 +240,27 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtasPerSm)
       return;
     }
     const int total = static_cast<int>(all);
-    ctas = min(static_cast<int>(gridDim.x), (total + kMinTiles - 1) / kMinTiles);
+    int ctas = min(static_cast<int>(gridDim.x), (total + kMinTiles - 1) / kMinTiles);
+    span = total;
+    per_group = ctas;
+    if (p.B == 1 && total > 0) {
+      const Request only = load_request<NT>(p, 0);
+      const int units = only.blocks * p.Hkv;
+      if (units <= ctas) {
+        span = only.tiles;
+        per_group = ctas / units;  // (at most 64, for fewer parts to join: no faster)
+        ctas = per_group * units;
+      }
+    }
     const int cta = blockIdx.x;
     if (cta >= ctas) {
       zero_padding();
       return;
     }
-    share = total / ctas;
-    extra = total - share * ctas;
-    cur.g = cta * share + min(cta, extra);
-    cur.end = cur.g + share + (cta < extra ? 1 : 0);
+    share = span / per_group;
+    extra = span - share * per_group;
+    cur.g = start_of(cta);
+    cur.end = cur.g + share + (cta % per_group < extra ? 1 : 0);
     if (before <= cur.g && cur.g < before + sum) {
       int b = b0, base = static_cast<int>(before);
       if (per > 1) r = load_request<NT>(p, b);
@@ -694,12 +712,12 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtasPerSm)
     if (s_flag[1]) {
       const int u0 = cur.base + cur.unit * cur.r.tiles, u1 = u0 + cur.r.tiles;
       auto owner = [&](int tile) {
-        const int longer = extra * (share + 1);
-        return tile < longer ? tile / (share + 1) : extra + (tile - longer) / share;
+        const int group = tile / span, longer = extra * (share + 1), t = tile - group * span;
+        return group * per_group + (t < longer ? t / (share + 1) : extra + (t - longer) / share);
       };
       const int c0 = owner(u0), n = owner(u1 - 1) - c0 + 1;
       // only the first of them can have had another unit before this one
-      const int first = c0 * 2 + (c0 * share + min(c0, extra) >= u0 ? 0 : 1);
+      const int first = c0 * 2 + (start_of(c0) >= u0 ? 0 : 1);
       auto slot_of = [&](int i) { return i == 0 ? first : (c0 + i) * 2; };
       // A warp, or several that share the parts, per row. Lanes hold the weights of 32 parts at a
       // time and 4 columns each (D = 64: the halves of the warp take every other part).
