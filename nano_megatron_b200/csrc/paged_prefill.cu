@@ -285,6 +285,11 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const Params p) 
         mma_commit(&k_empty[j & 1], leader);
         if (j > 0 && leader) mbar_arrive(&turn[1 - r]);
       }
+      if (!ok) {  // given up: wait (bounded) for the products on their way before TMEM is freed
+        mma_commit(&o_full[r], leader);
+        mbar_wait(&o_full[r], 0, p.status, kStatusAttnTimeout, nullptr);
+        __syncwarp();
+      }
     }
   } else if (warp >= 8) {
     // ------------------------------------------------------------------ converters
