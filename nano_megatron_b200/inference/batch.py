@@ -138,6 +138,11 @@ class BatchDecoder:
         if need > self.free:
             raise RuntimeError(f"the cache is out of pages: {need} needed, {self.free} free")
         ids = [t for s in slots for t in new_tokens[s]]
+        # (on CUDA a lookup outside the embedding would end the whole context)
+        vocab = self.model.original_vocab_size
+        if min(ids) < 0 or max(ids) >= vocab:
+            raise ValueError(f"token ids are 0..{vocab - 1}, the model's vocabulary; got "
+                             f"{min(ids) if min(ids) < 0 else max(ids)}")
         # one copy to the device: [token ids | context lengths | new lengths | last rows]
         ends, last = 0, []
         for s in slots:
