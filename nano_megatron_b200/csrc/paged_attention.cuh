@@ -6,9 +6,20 @@
 namespace nmb {
 namespace paged {
 
-// The running max only moves when a tile exceeds it by 2^8: most tiles then skip rescaling the
-// accumulator, and P <= 256 keeps its 11 bits in f16.
-constexpr float kLazy = 8.f;
+// Probabilities in f16. A row's running maximum M of t = score + log2 of the value scale moves when
+// a tile exceeds it by 2^4 (most tiles then skip rescaling the accumulator), and probabilities are
+// stored as 2^(t - M + 11): at most 2^15, with all 11 bits down to 2^-25 of 2^M and a quantum of
+// 2^-24 (error 2^-25) below that.
+constexpr float kLazy = 4.f;
+constexpr float kShift = 11.f;
+
+// That error of a key's probability matters only where the whole result is small: where M comes
+// from a key whose own value is next to nothing, because its page's scale was raised by another
+// key or because it just takes the weight. A row whose largest numerator is at least this times its
+// keys is within 2^-11 of it (keys * largest code * 2^-25); the others are computed again by
+// exact_row. A key with a code of 8 at the maximum is enough for 600,000 keys.
+template <bool INT8>
+constexpr float kResolved = (INT8 ? 127.f : 448.f) / 16384.f;
 
 struct Params {
   const __nv_bfloat16* q;
@@ -40,6 +51,90 @@ __device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// One row of a request over its first `keys` positions by one warp, with fp32 probabilities and
+// without the value scales in the maximum: the plain formula. For the few rows that the f16
+// probabilities cannot resolve (see kResolved), so simple rather than fast: a lane per key for the
+// scores, a lane per D / 32 columns for the sum. Leaves a row alone, and returns false, if all the
+// values it sees are zero: 0 is right already. Pages' value scales may differ by up to 2^100
+// (beyond, fp32 denominators lose keys that still count).
+template <int D, bool INT8>
+__device__ __forceinline__ bool exact_row(const Params& p, int b, int h, const __nv_bfloat16* q,
+                                          int keys, __nv_bfloat16* out, float* lse) {
+  constexpr int kCols = D / 32;
+  const int lane = threadIdx.x & 31;
+  const int* table = p.tables + b * p.table_stride;
+  // row of a key's codes, in units of D; -1 on a missing page
+  auto row_of = [&](int key) -> int64_t {
+    const int page = __ldg(table + (key >> p.page_shift));
+    if (page < 0 || page >= p.num_pages) return -1;
+    return ((static_cast<int64_t>(page) * p.Hkv + h) << p.page_shift) + (key & (p.ps - 1));
+  };
+  bool any = false;
+#pragma unroll 1
+  for (int k0 = 0; k0 < keys && !any; k0 += 32) {
+    const int64_t row = k0 + lane < keys ? row_of(k0 + lane) : -1;
+    uint32_t bits = 0;
+    for (int c = 0; c < D / 16 && row >= 0; ++c) {
+      const uint4 x = __ldg(reinterpret_cast<const uint4*>(p.v_codes + row * D) + c);
+      bits |= x.x | x.y | x.z | x.w;
+    }
+    any = __any_sync(0xffffffffu, (bits & (INT8 ? 0xffffffffu : 0x7f7f7f7fu)) != 0);
+  }
+  if (!any) return false;
+
+  float qv[kCols], x[kCols] = {}, m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int i = 0; i < kCols; ++i) qv[i] = __bfloat162float(q[lane * kCols + i]);
+#pragma unroll 1
+  for (int k0 = 0; k0 < keys; k0 += 32) {
+    const int64_t row = k0 + lane < keys ? row_of(k0 + lane) : -1;
+    const float ks = row >= 0 ? __ldg(p.k_scale + (row >> p.page_shift)) : 0.f;
+    const float vs = row >= 0 ? __ldg(p.v_scale + (row >> p.page_shift)) : 0.f;
+    float s = 0.f;
+#pragma unroll 1
+    for (int c = 0; c < D / 4; ++c) {
+      uint32_t f[2];
+      kv::decode4<INT8>(row >= 0 ? __ldg(reinterpret_cast<const uint32_t*>(p.k_codes + row * D) + c) : 0u,
+                        f[0], f[1]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 k2 = kv::f16x2_to_float2(f[e >> 1]);
+        const float qd = __shfl_sync(0xffffffffu, qv[e % kCols], (c * 4 + e) / kCols);
+        s = fmaf(qd, (e & 1 ? k2.y : k2.x) * ks, s);
+      }
+    }
+    s = row >= 0 ? s * p.scale_log2 : -INFINITY;
+    const float top = fmaxf(m, warp_max(s)), ref = top == -INFINITY ? 0.f : top;
+    const float w = ex2(s - ref), down = ex2(m - ref);
+    m = top;
+    l = fmaf(l, down, warp_sum(w));
+#pragma unroll
+    for (int i = 0; i < kCols; ++i) x[i] *= down;
+#pragma unroll 1
+    for (int k = 0; k < min(32, keys - k0); ++k) {
+      const int64_t at = __shfl_sync(0xffffffffu, row, k);
+      if (at < 0) continue;
+      const float wk = __shfl_sync(0xffffffffu, w, k), sk = __shfl_sync(0xffffffffu, vs, k);
+      const uint8_t* codes = p.v_codes + at * D + lane * kCols;
+      const uint32_t raw = kCols == 4 ? __ldg(reinterpret_cast<const uint32_t*>(codes))
+                                      : __ldg(reinterpret_cast<const uint16_t*>(codes));
+      uint32_t f[2];
+      kv::decode4<INT8>(raw, f[0], f[1]);
+#pragma unroll
+      for (int i = 0; i < kCols; ++i) {
+        const float2 v2 = kv::f16x2_to_float2(f[i >> 1]);
+        x[i] = fmaf(wk, (i & 1 ? v2.y : v2.x) * sk, x[i]);
+      }
+    }
+  }
+  const float inv = 1.f / l;
+  __syncwarp();                       // what this warp wrote there before
+#pragma unroll
+  for (int i = 0; i < kCols; i += 2)
+    *reinterpret_cast<uint32_t*>(out + lane * kCols + i) = pack_bf16x2(x[i] * inv, x[i + 1] * inv);
+  if (lse != nullptr && lane == 0) *lse = m + log2f(l);
+  return true;
+}
 
 }  // namespace paged
 }  // namespace nmb

@@ -5,9 +5,11 @@
 // with value codes c_j and value scales vs_j = 2^e_j (one per page and kv head). Because the
 // scales are powers of two, vs_j joins the logit: t_j = s_j + e_j, M = running max of t, and
 //   numerator += 2^(t_j - M) c_j,      denominator += 2^(t_j - M) 2^-e_j.
-// The f16 probabilities stay at most 2^8 (see kLazy) whatever the scales of different pages.
-// Codes of both formats are exact in f16, queries are scaled row by row by a power of two that
-// brings their largest magnitude to [1, 2), so the f16 products are exact; sums are fp32.
+// The f16 probabilities stay at most 2^15 whatever the scales of different pages (see kShift), and
+// rows that they cannot resolve are computed again in fp32 (kResolved). Codes of both formats are
+// exact in f16; queries are scaled row by row by a power of two that brings their largest magnitude
+// to [2^14, 2^15), so that elements down to 2^-31 of it are exact and smaller ones are off by at most
+// 2^-39 of it. Sums are fp32.
 //
 // Decode kernel (few query rows per request: decoding, short continuations). Bound by reading
 // the codes of K and V once: 128 requests of 512 to 4096 tokens, 8 kv heads of 128, take 123 us, 5.6 TB/s
@@ -69,7 +71,7 @@ struct Cfg {
   static constexpr int kRing = kStages * kStageBytes;
   static constexpr int kMerge = kWarps * 8 * 64 * 4;        // 8 rows by 64 columns at a time
   static constexpr int kStats = (kWarps + 1) * 8 * NT * 8;
-  static constexpr int kSmem = kRing + kMerge + kStats + kStages * 16 + kStages * 16 + 16;
+  static constexpr int kSmem = kRing + kMerge + kStats + kStages * 16 + kStages * 16 + 16 + 8 * NT * 4;
 };
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
@@ -171,6 +173,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtasPerSm)
   uint64_t* full = reinterpret_cast<uint64_t*>(s_info + S);
   uint64_t* empty = full + S;
   volatile int* s_flag = reinterpret_cast<volatile int*>(empty + S);         // abort, last
+  volatile int* s_ok = s_flag + 4;                                           // [row] see kResolved
 
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid / 32, 0);
   if (smem_u32(smem) & 1023u) {     // the swizzle pattern needs 1024-byte alignment
@@ -402,8 +405,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtasPerSm)
       }
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-      // exponent of the row's largest magnitude (fmaxf drops NaN; infinity keeps 126)
-      const int e = min(max(kv::exponent_of(amax), -100), 126);
+      // the row's largest magnitude goes to [2^14, 2^15) (fmaxf drops NaN; infinity stays)
+      const int e = min(max(kv::exponent_of(amax) - 14, -100), 113);
       const float down = kv::pow2i(-e), up = kv::pow2i(e) * p.scale_log2;
       const int see = live ? cur.r.kv - cur.r.nq + tok + 1 : 0;
 #pragma unroll
@@ -527,8 +530,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtasPerSm)
       uint32_t pb[2][NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const float r0 = m_run[nt][0] == -INFINITY ? 0.f : m_run[nt][0];
-        const float r1 = m_run[nt][1] == -INFINITY ? 0.f : m_run[nt][1];
+        const float r0 = m_run[nt][0] == -INFINITY ? 0.f : m_run[nt][0] - kShift;
+        const float r1 = m_run[nt][1] == -INFINITY ? 0.f : m_run[nt][1] - kShift;
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt) {
           const float p0 = ex2(s[mt][nt][0] - r0), p1 = ex2(s[mt][nt][1] - r1);
@@ -647,9 +650,18 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtasPerSm)
           l = fmaf(st.y, ex2(st.x - ref), l);
         }
         corr[nt][c] = ex2(m_run[nt][c] - ref);
-        if (warp == 0 && g8 == 0) s_tot[row] = make_float2(m, l);
+        if (warp == 0 && g8 == 0) {
+          s_tot[row] = make_float2(m, l);
+          s_ok[row] = 0;
+        }
       }
     const bool whole = cur.n == cur.r.tiles;
+    // Keys that a token's rows see, and whether part of a row's numerator is large enough for them.
+    auto keys_of = [&](int tok) { return min(cur.r.kv, cur.r.kv - cur.r.nq + tok + 1); };
+    auto resolved = [&](const float4& x, float l, int tok) {
+      const float top = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+      return top >= kResolved<INT8> * keys_of(tok) || !(l > 0.f && l < INFINITY);
+    };
     const int slot = blockIdx.x * 2 + (first_run ? 0 : 1);
     float* part = p.part + static_cast<int64_t>(slot) * (kRows * D);
     constexpr int kParts = D / 64;  // 64 columns at a time; at D = 128 those of even, then odd g8
@@ -686,20 +698,19 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtasPerSm)
           const int64_t at = static_cast<int64_t>(cur.r.q0 + tok) * p.Hq + head;
           *reinterpret_cast<uint2*>(p.o + at * D + q * 4) =
               make_uint2(pack_bf16x2(x.x * inv, x.y * inv), pack_bf16x2(x.z * inv, x.w * inv));
+          if (resolved(x, tot.y, tok)) s_ok[row] = 1;
           if (p.lse != nullptr && q == 0)
-            p.lse[at] = tot.y == 0.f ? -INFINITY : tot.x + log2f(tot.y);
+            p.lse[at] = tot.y == 0.f ? -INFINITY : tot.x - kShift + log2f(tot.y);
         } else {
           *reinterpret_cast<float4*>(part + row * D + q * 4) = x;
           if (q == 0) p.part_ml[slot * kRows + row] = tot;
         }
       }
     }
-    if (whole) continue;
-
     // ---- a unit shared with other CTAs: the last to finish adds the parts up in CTA order
     sync_all();
     const int rpt = (p.G + kRows - 1) / kRows;
-    if (tid == 0) {
+    if (tid == 0 && !whole) {
       int* counter = p.counters + (static_cast<int64_t>(h) * p.T + cur.r.q0) * rpt + rb;
       __threadfence();              // the barrier and this fence publish the whole CTA's part
       const int before = atomicAdd(counter, cur.n);
@@ -708,8 +719,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtasPerSm)
       __threadfence();
       s_flag[1] = last;
     }
-    sync_all();
-    if (s_flag[1]) {
+    if (!whole) sync_all();
+    if (!whole && s_flag[1]) {
       const int u0 = cur.base + cur.unit * cur.r.tiles, u1 = u0 + cur.r.tiles;
       auto owner = [&](int tile) {
         const int group = tile / span, longer = extra * (share + 1), t = tile - group * span;
@@ -793,7 +804,19 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtasPerSm)
         if (odd == 0)
           *reinterpret_cast<uint2*>(p.o + at * D + col) =
               make_uint2(pack_bf16x2(x.x * inv, x.y * inv), pack_bf16x2(x.z * inv, x.w * inv));
-        if (p.lse != nullptr && lane == 0) p.lse[at] = l == 0.f ? -INFINITY : m + log2f(l);
+        if (resolved(x, l, tok)) s_ok[row] = 1;
+        if (p.lse != nullptr && lane == 0) p.lse[at] = l == 0.f ? -INFINITY : m - kShift + log2f(l);
+      }
+      sync_all();
+    }
+    if (whole || s_flag[1]) {
+#pragma unroll 1
+      for (int row = warp; row < rows; row += kWarps) {
+        if (s_ok[row]) continue;
+        const int tok = (rb * kRows + row) / p.G, g = (rb * kRows + row) - tok * p.G;
+        const int64_t at = static_cast<int64_t>(cur.r.q0 + tok) * p.Hq + h * p.G + g;
+        exact_row<D, INT8>(p, cur.b, h, p.q + (cur.r.q0 + tok) * p.q_row + (h * p.G + g) * p.q_head,
+                           keys_of(tok), p.o + at * D, p.lse == nullptr ? nullptr : p.lse + at);
       }
     }
   }

@@ -1,7 +1,7 @@
 // Attention over the 8-bit paged cache for requests with many new tokens (prompts and chunks of
 // them) on the tensor cores (tcgen05 + TMEM). Same mathematics as the decode kernel
-// (paged_attention.cu): log2 of the power-of-two value scale joins the logit, codes and queries
-// are exact in f16, sums are fp32.
+// (paged_decode.cuh): log2 of the power-of-two value scale joins the logit, codes and queries
+// go to f16 (which holds both), sums are fp32.
 //
 // Bound by the tensor cores and the exponentials: 128 keys cost a pair of 128-row tiles about
 // 2,100 cycles of tcgen05.mma at the nominal rate and as many of ex2. Measured: about 5,000, the chain
@@ -12,7 +12,7 @@
 // share every converted key) of one request and kv head, 512 threads:
 //   warps 0-3, 4-7 : softmax of tile 0 / 1, a thread per row: loads S (tcgen05.ld), online softmax
 //                    in base 2, writes P (f16) over S in TMEM, rescales O there when the maximum
-//                    grows by more than 2^8, and stores the result at the end;
+//                    grows by more than 2^4, and stores the result at the end;
 //   warps 8-11     : converters: cache codes from global memory (prefetched into registers one
 //                    tile ahead) to f16 tiles in shared memory, in the K-major / MN-major
 //                    128-byte-swizzled layouts that tcgen05.mma reads, two stages each of K and V;
@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const Params p) 
     const int first_limit = kv - n + tok0 + rt * tpt + 1;     // of the tile's first row
     float row_scale = 0.f;
     if (rt < rts) {
-      // this row's query, scaled to [1, 2) by a power of two, as f16
+      // this row's query, scaled to [2^14, 2^15) by a power of two, as f16
       const __nv_bfloat16* src = p.q + (q0 + tok) * p.q_row + (h * p.G + head) * p.q_head;
       uint4 raw[D / 8];
       float amax = 0.f;
@@ -423,7 +423,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const Params p) 
         for (int e = 0; e < 4; ++e)
           amax = fmaxf(amax, fmaxf(fabsf(bf16_lo(w[e])), fabsf(bf16_hi(w[e]))));
       }
-      const int e = min(max(kv::exponent_of(amax), -100), 126);
+      const int e = min(max(kv::exponent_of(amax) - 14, -100), 113);
       const float down = p.scale_log2 < 0.f ? -kv::pow2i(-e) : kv::pow2i(-e);
       row_scale = kv::pow2i(e) * fabsf(p.scale_log2);
 #pragma unroll
@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const Params p) 
           }
         }
       }
-      const float ref = m_run == -INFINITY ? 0.f : m_run;
+      const float ref = m_run == -INFINITY ? 0.f : m_run - kShift;
 #pragma unroll
       for (int g = 0; g < 8; ++g) {
         const float4 f = info[g];
@@ -541,12 +541,15 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const Params p) 
         }
       }
       if (ok) {
+        float top = 0.f;
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
           if (tiles > 0) {
             tmem_ld_32x32b_x32(tO + c * 32, o);
             tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) top = fmaxf(top, fabsf(__uint_as_float(o[e])));
           }
           if (!INT8 && nan_cols[c] != 0)
 #pragma unroll
@@ -566,7 +569,22 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const Params p) 
             }
           }
         }
-        if (live && p.lse != nullptr) p.lse[at] = l_run == 0.f ? -INFINITY : m_run + log2f(l_run);
+        if (live && p.lse != nullptr)
+          p.lse[at] = l_run == 0.f ? -INFINITY : m_run - kShift + log2f(l_run);
+        // the last row first: if it sees no value but zeros, neither do the others
+        const int keys_seen = min(limit, kv);
+        uint32_t again = __ballot_sync(0xffffffffu, l_run > 0.f && l_run < INFINITY &&
+                                                        top < kResolved<INT8> * keys_seen);
+#pragma unroll 1
+        while (again) {
+          const int i = 31 - __clz(again);
+          again ^= 1u << i;
+          const int64_t row_at = __shfl_sync(0xffffffffu, at, i);
+          const int64_t row_q = __shfl_sync(0xffffffffu, (q0 + tok) * p.q_row + (h * p.G + head) * p.q_head, i);
+          if (!exact_row<D, INT8>(p, b, h, p.q + row_q, __shfl_sync(0xffffffffu, keys_seen, i),
+                                  p.o + row_at * D, p.lse == nullptr ? nullptr : p.lse + row_at))
+            break;
+        }
       }
     }
   }

@@ -1,0 +1,109 @@
+"""Edges of the batched-serving kernels against plain 64-bit computations.
+
+Tolerances as in ``test_serving_ops_gpu``: attention rounds its output once to bf16 (2^-8 of the
+value) and each probability to f16 (under 2^-10 of the row's largest output in sum).
+"""
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from test_serving_ops_gpu import DEV, E4M3, INT8, _cache, _oracle, ints  # noqa: E402
+
+from nano_megatron_b200.ops import check_status, serving  # noqa: E402
+
+BOUND = 2.0 ** -8 + 2.0 ** -10
+
+
+def _compare(q, cache, tables, starts, kv, max_new):
+    lse = torch.empty(q.shape[:2], device=DEV)
+    got = serving.paged_attention(q, cache, tables, ints(starts), ints(kv), max_new=max_new, lse=lse)
+    torch.cuda.synchronize()
+    check_status(torch.device(DEV))
+    want, want_lse = _oracle(q, cache, tables, starts, kv, q.shape[2] ** -0.5)
+    top = want.abs().amax(-1, keepdim=True)
+    worst = ((got.double() - want).abs() / top.clamp(min=1e-300)).max().item()
+    assert worst <= BOUND, worst
+    inf = torch.isinf(want_lse)
+    assert torch.equal(torch.isinf(lse), inf)
+    assert bool(((lse.double() - want_lse)[~inf].abs() <= 2.0 ** -16 + want_lse[~inf].abs() * 2.0 ** -18).all())
+
+
+def _rows_and_cache(n, new, Hq, H, D, page, dtype, special):
+    """One request of `n` keys, the last `new` of them new. Queries point along one direction, so
+    that ``special(k, v, direction)`` can give single keys a chosen score; values are normal."""
+    g = torch.Generator(device=DEV).manual_seed(n + new)
+    u = torch.nn.functional.normalize(torch.randn(D, generator=g, device=DEV), dim=0)
+    q = (4.0 * u + 0.1 * torch.randn(new, Hq, D, generator=g, device=DEV)).bfloat16()
+    k = torch.randn(n, H, D, generator=g, device=DEV)
+    k -= (k @ u)[..., None] * u                          # ordinary keys: scores near zero
+    v = torch.randn(n, H, D, generator=g, device=DEV)
+    special(k, v, u)
+    pages = -(-n // page)
+    cache = _cache(pages + 1, H, D, page, dtype)
+    ids = torch.randperm(pages, generator=torch.Generator().manual_seed(n)).tolist()
+    serving.append_kv(cache, k.bfloat16(), v.bfloat16(),
+                      ints([[p, i * page, 0, min(page, n - i * page)] for i, p in enumerate(ids)]))
+    return q, cache, ints([ids])
+
+
+# (keys, new rows, query heads, kv heads): one row on one block and on many, a few rows, 16-row
+# units, prompts in the other kernel
+SHAPES = [(300, 1, 4, 2), (5000, 1, 4, 1), (200, 3, 2, 2), (150, 5, 8, 2), (400, 130, 4, 2)]
+
+
+@pytest.mark.parametrize("dtype", [E4M3, INT8])
+@pytest.mark.parametrize("D,page", [(64, 16), (128, 64)])
+@pytest.mark.parametrize("n,new,Hq,H", SHAPES)
+@pytest.mark.parametrize("power", [16, 20, 24, 30])
+def test_value_outlier_of_low_weight(dtype, D, page, n, new, Hq, H, power):
+    """One visible value of 2^power whose key has a score of about -90 (a weight under 1e-25): its page's
+    scale is large, yet the other pages decide the result."""
+    def special(k, v, u):
+        k[7], v[7, :, 3] = -22.5 * D ** 0.5 * u, 2.0 ** power
+
+    q, cache, tables = _rows_and_cache(n, new, Hq, H, D, page, dtype, special)
+    _compare(q, cache, tables, [0, new], [n], new)
+
+
+@pytest.mark.parametrize("dtype", [E4M3, INT8])
+@pytest.mark.parametrize("D,page", [(64, 16), (128, 64)])
+@pytest.mark.parametrize("n,new,Hq,H", [s for s in SHAPES if s[1] > 1])
+@pytest.mark.parametrize("power", [16, 24, 30])
+def test_value_outlier_hidden_by_causality(dtype, D, page, n, new, Hq, H, power):
+    """The last position's value is 2^power: only the last row sees it, the others share its page's
+    scale."""
+    def special(k, v, u):
+        v[-1, :, 3] = 2.0 ** power
+
+    q, cache, tables = _rows_and_cache(n, new, Hq, H, D, page, dtype, special)
+    _compare(q, cache, tables, [0, new], [n], new)
+
+
+@pytest.mark.parametrize("dtype", [E4M3, INT8])
+@pytest.mark.parametrize("D,page", [(64, 16), (128, 64)])
+@pytest.mark.parametrize("n,new,Hq,H", SHAPES)
+@pytest.mark.parametrize("bits", [12, 20, 30, 40, 60])
+def test_key_that_takes_all_the_weight_but_has_no_value(dtype, D, page, n, new, Hq, H, bits):
+    """A first key whose score is `bits` powers of two above the others and whose value is zero:
+    the result is the others' sum, at 2^-bits of the largest probability."""
+    def special(k, v, u):
+        k[0], v[0] = bits * math.log(2.0) / 4.0 * D ** 0.5 * u, 0.0
+
+    q, cache, tables = _rows_and_cache(n, new, Hq, H, D, page, dtype, special)
+    _compare(q, cache, tables, [0, new], [n], new)
+
+
+@pytest.mark.parametrize("dtype", [E4M3, INT8])
+@pytest.mark.parametrize("D,page", [(64, 16), (128, 64)])
+@pytest.mark.parametrize("n,new,Hq,H", SHAPES)
+def test_values_of_zero(dtype, D, page, n, new, Hq, H):
+    def special(k, v, u):
+        v.zero_()
+
+    q, cache, tables = _rows_and_cache(n, new, Hq, H, D, page, dtype, special)
+    o = serving.paged_attention(q, cache, tables, ints([0, new]), ints([n]), max_new=new)
+    assert o.abs().max() == 0
