@@ -21,8 +21,8 @@ from dataclasses import dataclass
 import torch
 
 from nano_megatron_b200.nn.rotary import rope_inv_freq
+from nano_megatron_b200.ops import check_status, serving
 from nano_megatron_b200.ops import functional as F
-from nano_megatron_b200.ops import serving
 
 from .artifact import InferenceArtifact
 from .generation import (
@@ -119,7 +119,10 @@ class BatchDecoder:
     @torch.inference_mode()
     def step(self, new_tokens: dict[int, Sequence[int]]) -> torch.Tensor:
         """Append ``new_tokens[slot]`` to each request named; returns the scores of the last
-        token of each ([len(new_tokens), vocabulary], in the order of the slots' numbers)."""
+        token of each ([len(new_tokens), vocabulary], in the order of the slots' numbers).
+
+        Does not wait for the GPU; on CUDA ``check_status`` says, once the scores are read, whether
+        a kernel gave up and they are unfinished."""
         slots = sorted(new_tokens)
         if not slots:
             raise ValueError("a step needs at least one request")
@@ -307,6 +310,8 @@ def generate_batch(artifact: InferenceArtifact, model, prompts: Sequence[str], *
             slots = sorted(pending)
             scores = held.apply(scores, slots, [dec.lengths[s] for s in slots],
                                 [pending[s][-1] for s in slots]).cpu()
+            if dec.device.type == "cuda":
+                check_status(dec.device)
             pending = {}
             for row, slot in zip(scores, slots):
                 i = serving_slots[slot]

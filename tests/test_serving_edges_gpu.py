@@ -107,3 +107,35 @@ def test_values_of_zero(dtype, D, page, n, new, Hq, H):
     q, cache, tables = _rows_and_cache(n, new, Hq, H, D, page, dtype, special)
     o = serving.paged_attention(q, cache, tables, ints([0, new]), ints([n]), max_new=new)
     assert o.abs().max() == 0
+
+
+def test_generation_stops_at_a_kernels_status():
+    """A kernel that gave up (here: its status word, set by hand) leaves its output unfinished:
+    nothing is sampled from it."""
+    from test_batch_generation_gpu import _model
+
+    from nano_megatron_b200.inference import generate_batch
+    from nano_megatron_b200.ops import status_word
+
+    model, cfg = _model(DEV, torch.bfloat16, 4, 2)
+
+    class Numbers:
+        eos_token_id = 8191
+
+        def encode(self, text, add_bos, add_eos):
+            return [int(x) for x in text.split()]
+
+        def decode(self, ids, skip_special_tokens):
+            return " ".join(map(str, ids))
+
+    from types import SimpleNamespace
+    art = SimpleNamespace(tokenizer=Numbers(), model_config=cfg.model)
+    word = status_word(torch.device(DEV))
+    kw = dict(device=torch.device(DEV), max_new_tokens=2, temperature=0.0)
+    try:
+        word.fill_(0x201)
+        with pytest.raises(RuntimeError, match="attention wait timed out"):
+            generate_batch(art, model, ["1 2 3"], **kw)
+    finally:
+        word.zero_()
+    assert len(generate_batch(art, model, ["1 2 3"], **kw)[0].generated_token_ids) == 2
