@@ -15,7 +15,7 @@ not depend on what else is in the batch (up to the rounding of differently shape
 from __future__ import annotations
 
 import math
-from collections.abc import Sequence
+from collections.abc import Iterable, Sequence
 from dataclasses import dataclass
 
 import torch
@@ -42,14 +42,15 @@ class LogitRules:
 
     ``repetition`` > 1 makes tokens of the prompt and the completion less likely,
     ``presence`` / ``frequency`` subtract a constant once / per occurrence in the completion,
-    ``bias`` adds to single tokens, ``allowed`` restricts sampling to a set of token ids.
+    ``bias`` adds to single tokens, ``allowed`` restricts sampling to a set of token ids (any
+    iterable, kept as a tuple; at least one).
     """
 
     repetition: float = 1.0
     presence: float = 0.0
     frequency: float = 0.0
     bias: dict[int, float] | None = None
-    allowed: Sequence[int] | None = None
+    allowed: Iterable[int] | None = None
 
     def __post_init__(self) -> None:
         if not (math.isfinite(self.repetition) and self.repetition > 0.0):
@@ -57,6 +58,10 @@ class LogitRules:
         for name in ("presence", "frequency"):
             if not math.isfinite(getattr(self, name)):
                 raise ValueError(f"{name} must be finite")
+        if self.allowed is not None:
+            object.__setattr__(self, "allowed", tuple(self.allowed))
+            if not self.allowed:
+                raise ValueError("allowed is empty: no token could be sampled (None allows all)")
 
     @property
     def empty(self) -> bool:
@@ -317,6 +322,8 @@ def generate_batch(artifact: InferenceArtifact, model, prompts: Sequence[str], *
                 i = serving_slots[slot]
                 nxt = sample_next_token(row, temperature=float(temperature), top_p=float(top_p),
                                         top_k=top_k, generator=gens[i])
+                if not math.isfinite(float(row[nxt])):   # the largest, at temperature 0
+                    raise RuntimeError(f"no token left to sample for prompt {i}: no score is finite")
                 new[i].append(nxt)
                 if nxt == tok.eos_token_id:
                     stop[i] = "eos"

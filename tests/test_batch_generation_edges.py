@@ -1,5 +1,7 @@
 """Edges of batched generation and of the serving operators' CPU forms."""
 
+import math
+
 import pytest
 import torch
 from test_batch_generation import CPU, PROMPTS, _artifact, _batch  # noqa: F401
@@ -21,3 +23,32 @@ def test_token_ids_outside_the_vocabulary_are_refused(tmp_path, bad):
     with pytest.raises(ValueError, match="vocabulary"):
         dec.step({0: [3], 1: [4, model.original_vocab_size if bad == "vocab" else bad, 7]})
     assert _state(dec) == before and torch.equal(dec.tables, tables)
+
+
+def test_an_empty_allowed_set_is_refused():
+    from nano_megatron_b200.inference import LogitRules
+
+    for nothing in ((), [], set(), iter(())):
+        with pytest.raises(ValueError, match="allowed"):
+            LogitRules(allowed=nothing)
+
+
+def test_allowed_may_be_any_iterable(tmp_path):
+    """An iterator is not used up by the checks of its ids."""
+    from nano_megatron_b200.inference import LogitRules
+
+    art, model = _artifact(tmp_path)
+    want = _batch(art, model, rules=LogitRules(allowed=[11, 12, 40]))
+    got = _batch(art, model, rules=LogitRules(allowed=iter([11, 12, 40])))
+    assert [r.generated_token_ids for r in got] == [r.generated_token_ids for r in want]
+    assert {t for r in got for t in r.generated_token_ids} <= {11, 12, 40}
+
+
+@pytest.mark.parametrize("temperature", [0.0, 0.8])
+def test_rules_that_leave_no_token_stop_generation(tmp_path, temperature):
+    from nano_megatron_b200.inference import LogitRules
+
+    art, model = _artifact(tmp_path)
+    rules = LogitRules(allowed=[7, 9], bias={7: -math.inf, 9: -math.inf})
+    with pytest.raises(RuntimeError, match="no token"):
+        _batch(art, model, rules=rules, temperature=temperature)
