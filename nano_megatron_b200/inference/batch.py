@@ -42,7 +42,7 @@ class LogitRules:
 
     ``repetition`` > 1 makes tokens of the prompt and the completion less likely,
     ``presence`` / ``frequency`` subtract a constant once / per occurrence in the completion,
-    ``bias`` adds to single tokens, ``allowed`` restricts sampling to a set of token ids (any
+    ``bias`` adds to single tokens (-inf bans one), ``allowed`` restricts sampling to a set of token ids (any
     iterable, kept as a tuple; at least one).
     """
 
@@ -58,6 +58,9 @@ class LogitRules:
         for name in ("presence", "frequency"):
             if not math.isfinite(getattr(self, name)):
                 raise ValueError(f"{name} must be finite")
+        for t, x in (self.bias or {}).items():
+            if math.isnan(x) or x == math.inf:
+                raise ValueError(f"bias of token {t} must be a number or -inf, not {x}")
         if self.allowed is not None:
             object.__setattr__(self, "allowed", tuple(self.allowed))
             if not self.allowed:

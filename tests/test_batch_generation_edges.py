@@ -52,3 +52,12 @@ def test_rules_that_leave_no_token_stop_generation(tmp_path, temperature):
     rules = LogitRules(allowed=[7, 9], bias={7: -math.inf, 9: -math.inf})
     with pytest.raises(RuntimeError, match="no token"):
         _batch(art, model, rules=rules, temperature=temperature)
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_biases_of_nan_or_infinity_are_refused(value):
+    from nano_megatron_b200.inference import LogitRules
+
+    with pytest.raises(ValueError, match="bias"):
+        LogitRules(bias={3: 1.0, 4: value})
+    assert LogitRules(bias={3: -math.inf}).bias == {3: -math.inf}
