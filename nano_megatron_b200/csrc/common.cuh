@@ -50,6 +50,7 @@ enum StatusCode : int {
   kStatusGemmEpilogueTimeout = 0x103,
   kStatusAttnTimeout = 0x201,
   kStatusSmemAlignment = 0x202,
+  kStatusAttnTiles = 0x203,
   kStatusPeerFlagTimeout = 0x301,
   kStatusPeerBarrierTimeout = 0x302,
   kStatusReplicaFlagTimeout = 0x401,

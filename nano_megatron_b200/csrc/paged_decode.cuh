@@ -238,8 +238,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtasPerSm)
       if (i < warp) before += s_scan[i];
       all += s_scan[i];
     }
-    if (all > 0x3fffffff) {         // more than any memory holds
-      if (tid == 0) record_status(p.status, kStatusAttnTimeout);
+    // Tiles are counted once per block of rows: groups over 128 heads, whose prompts come here too,
+    // reach this with long ones (160 heads of a group, 4 groups, a prompt of 32k tokens).
+    if (all > 0x3fffffff) {
+      if (tid == 0) record_status(p.status, kStatusAttnTiles);
       return;
     }
     const int total = static_cast<int>(all);

@@ -51,6 +51,7 @@ STATUS_NAMES = {
     0x103: "GEMM epilogue wait timed out",
     0x201: "attention wait timed out",
     0x202: "shared memory was not aligned as a kernel needs it",
+    0x203: "attention over the paged cache: too many key tiles for one call",
     0x301: "peer flag wait timed out",
     0x302: "peer barrier wait timed out",
     0x401: "data-parallel replica flag wait timed out",

@@ -211,6 +211,9 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, tables: torch.Tensor,
     (table entry -1) are not seen. NaN in a position reaches the rows that see it and no others.
     ``lse`` (fp32 [tokens, heads]) receives the base-2 log-sum-exp of the scaled scores, -inf for
     rows that see nothing. Value scales of one request's pages may differ by up to 2**100.
+
+    On CUDA, more than 2**30 tiles of 32 keys by 16 rows in one call (prompts of more than 128
+    heads per kv head) leave the output unwritten and a status for ``check_status``.
     """
     D = cache.k_pages.shape[3]
     scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(D)

@@ -139,3 +139,20 @@ def test_generation_stops_at_a_kernels_status():
     finally:
         word.zero_()
     assert len(generate_batch(art, model, ["1 2 3"], **kw)[0].generated_token_ids) == 2
+
+
+def test_a_step_of_too_many_key_tiles_has_its_own_status():
+    """Groups over 128 heads always take the decode kernel, which counts its key tiles in 31 bits."""
+    from nano_megatron_b200.ops import status_word
+
+    cache = serving.PagedKV.create(1, 1, 64, page_size=128)
+    n, heads, keys = 16384, 130, 300 * 1024
+    q = torch.zeros(n, heads, 64, device=DEV, dtype=torch.bfloat16)
+    tables = torch.zeros(1, keys // 128, dtype=torch.int32, device=DEV)
+    word = status_word(torch.device(DEV))
+    try:
+        serving.paged_attention(q, cache, tables, ints([0, n]), ints([keys]), max_new=n)
+        with pytest.raises(RuntimeError, match="key tiles"):
+            check_status(torch.device(DEV))
+    finally:
+        word.zero_()
