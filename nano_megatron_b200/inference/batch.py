@@ -286,6 +286,9 @@ def generate_batch(artifact: InferenceArtifact, model, prompts: Sequence[str], *
         for t in list(rules[i].bias or ()) + list(rules[i].allowed or ()):
             if not 0 <= t < vocab:
                 raise ValueError(f"token id {t} of the rules is outside the vocabulary ({vocab})")
+        if model.embedding.weight.is_cuda and len(rules[i].bias or ()) > serving.MAX_BIAS:
+            raise ValueError(f"at most {serving.MAX_BIAS} biases a prompt on CUDA, "
+                             f"prompt {i} has {len(rules[i].bias)}")
     longest = max(len(p) for p in ids) + max_new_tokens
     dec = BatchDecoder(model, max_requests=min(max_batch, len(prompts)), max_len=longest,
                        num_pages=num_pages, page_size=page_size,

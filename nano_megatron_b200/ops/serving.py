@@ -32,6 +32,7 @@ from ._ext import lib, status_word
 
 PAGE_SIZES = (16, 32, 64, 128)
 CODE_TYPES = {torch.float8_e4m3fn: 448.0, torch.int8: 127.0}
+MAX_BIAS = 1024               # biases of a row that the kernel of ``adjust_logits`` takes
 _SCALE_EXP = 60
 
 
@@ -273,7 +274,8 @@ def adjust_logits(logits: torch.Tensor, history: torch.Tensor, history_lens: tor
 
     * tokens that occur in the history: score / ``repetition[b]`` if positive, else times it;
     * tokens generated ``c > 0`` times: minus ``frequency[b] * c + presence[b]``;
-    * ``bias[b, i]`` is added to token ``bias_ids[b, i]`` (int32; -1 = unused; repeated ids add);
+    * ``bias[b, i]`` is added to token ``bias_ids[b, i]`` (int32; -1 = unused; repeated ids add;
+      on CUDA at most ``MAX_BIAS`` a row);
     * tokens whose bit in ``allowed`` (int32 [B, ceil(V / 32)], bit ``v % 32`` of word
       ``v // 32``) is 0 become -inf, whatever their score.
     """

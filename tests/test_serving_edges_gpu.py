@@ -156,3 +156,25 @@ def test_a_step_of_too_many_key_tiles_has_its_own_status():
             check_status(torch.device(DEV))
     finally:
         word.zero_()
+
+
+def test_more_biases_than_the_kernel_takes_are_refused_before_the_first_step():
+    from types import SimpleNamespace
+
+    from test_batch_generation_gpu import _model
+
+    from nano_megatron_b200.inference import LogitRules, generate_batch
+    from nano_megatron_b200.ops import lib
+
+    model, cfg = _model(DEV, torch.bfloat16, 4, 2)
+    words = SimpleNamespace(eos_token_id=8191, encode=lambda t, add_bos, add_eos: [1, 2, 3],
+                            decode=lambda ids, skip_special_tokens: "")
+    art = SimpleNamespace(tokenizer=words, model_config=cfg.model)
+    kw = dict(device=torch.device(DEV), max_new_tokens=2, temperature=0.0)
+    before = lib().launch_count()
+    with pytest.raises(ValueError, match=str(serving.MAX_BIAS)):
+        generate_batch(art, model, ["a", "b"],
+                       rules=[LogitRules(), LogitRules(bias={t: 0.5 for t in range(serving.MAX_BIAS + 1)})], **kw)
+    assert lib().launch_count() == before
+    most = LogitRules(bias={t: 100.0 for t in range(serving.MAX_BIAS)})
+    assert max(generate_batch(art, model, ["a"], rules=most, **kw)[0].generated_token_ids) < serving.MAX_BIAS
