@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
   int64_t sum = 0, total;
   for (int b = b0; b < b1; ++b) sum += min(max(p.fresh[b], 0), p.T);
   int64_t at = block_scan(sum, warp_sums, total);
-  int touch = 0, fresh = 0;
+  int touch = 0, fresh = 0, beyond = 0;
   for (int b = b0; b < b1; ++b) {
     // rows past the T that the outputs hold are dropped
     const int row = static_cast<int>(min(at, static_cast<int64_t>(p.T))), n = min(max(p.fresh[b], 0), p.T - row);
@@ -82,13 +82,18 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
     const int ctx = context_of(b);
     s_row[b] = row;
     s_touch[b] = n > 0 ? ((ctx + n - 1) >> p.page_shift) - (ctx >> p.page_shift) + 1 : 0;
-    s_fresh[b] = ((ctx + n + ps - 1) >> p.page_shift) - ((ctx + ps - 1) >> p.page_shift);
+    // new pages that the table has columns for; the others stay in the free list
+    const int old = (ctx + ps - 1) >> p.page_shift, after = (ctx + n + ps - 1) >> p.page_shift;
+    s_fresh[b] = max(min(after, p.width) - old, 0);
     touch += s_touch[b];
     fresh += s_fresh[b];
+    beyond += after - old - s_fresh[b];
   }
   int64_t touch_total, fresh_total;
   int touch_at = static_cast<int>(block_scan(touch, warp_sums, touch_total));
-  int fresh_at = static_cast<int>(block_scan(fresh, warp_sums, fresh_total));
+  // two sums in one scan, each below 2^31: new pages in the low half, those beyond the tables above
+  int fresh_at = static_cast<int>(
+      block_scan(fresh + (static_cast<int64_t>(beyond) << 32), warp_sums, fresh_total));
   for (int b = b0; b < b1; ++b) {
     const int t = s_touch[b], f = s_fresh[b];
     s_touch[b] = touch_at;
@@ -149,7 +154,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
       p.q_starts[p.B] = s_row[p.B];
       const int need = s_fresh[p.B];
       *p.free_out = max(have - need, 0);
-      *p.missing = max(need - have, 0);
+      *p.missing = max(need - have, 0) + static_cast<int>(fresh_total >> 32);
     }
   }
 }

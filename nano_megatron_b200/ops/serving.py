@@ -71,8 +71,9 @@ class StepPlan(NamedTuple):
     ``positions`` / ``slots`` [num_tokens]: position in its request and cache slot
     (``page * page_size + offset``) of each row, 0 / -1 for rows past the last request;
     ``touched`` [U, 4]: (page, first row, first offset, rows) of every page that gets rows,
-    (-1, 0, 0, 0) past the last; ``free_count`` [1]: free pages left; ``missing`` [1]: pages
-    that the free list could not give (their rows have slot -1 and are not cached).
+    (-1, 0, 0, 0) past the last; ``free_count`` [1]: free pages left; ``missing`` [1]: new
+    pages that the free list could not give or a table has no column for (their rows have slot -1
+    and are not cached; pages without a column stay in the free list).
     """
 
     q_starts: torch.Tensor
@@ -107,17 +108,18 @@ def plan_step(context_lens: torch.Tensor, new_lens: torch.Tensor, tables: torch.
     positions, slots = [0] * num_tokens, [-1] * num_tokens
     touched, starts, kv = [], [0], []
     have = min(max(int(free_count), 0), free_pages.numel())
-    taken = 0
+    taken = beyond = 0
     for b in range(B):
         ctx = max(int(context_lens[b]), 0)
         row = starts[-1]
         n = min(max(int(new_lens[b]), 0), num_tokens - row)
         old = -(-ctx // page_size)
         for lp in range(old, -(-(ctx + n) // page_size)):
-            page = int(free_pages[have - 1 - taken]) if taken < have else -1
+            if lp >= width:
+                beyond += 1
+                continue
+            tables[b, lp] = int(free_pages[have - 1 - taken]) if taken < have else -1
             taken += 1
-            if lp < width:
-                tables[b, lp] = page
         at = ctx
         while at < ctx + n:
             lp = at // page_size
@@ -138,7 +140,7 @@ def plan_step(context_lens: torch.Tensor, new_lens: torch.Tensor, tables: torch.
 
     return StepPlan(ints(starts), ints(kv), ints(positions), ints(slots),
                     ints(touched).reshape(room, 4), ints([max(have - taken, 0)]),
-                    ints([max(taken - have, 0)]))
+                    ints([max(taken - have, 0) + beyond]))
 
 
 def _scale_exponent(amax: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:

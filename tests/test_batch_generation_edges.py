@@ -61,3 +61,40 @@ def test_biases_of_nan_or_infinity_are_refused(value):
     with pytest.raises(ValueError, match="bias"):
         LogitRules(bias={3: 1.0, 4: value})
     assert LogitRules(bias={3: -math.inf}).bias == {3: -math.inf}
+
+
+def narrow_table_plans(device):
+    """Plans whose tables have no room for all new pages, with more free pages than needed."""
+    from nano_megatron_b200.ops import serving
+
+    def ints(v):
+        return torch.tensor(v, dtype=torch.int32, device=device)
+
+    for contexts, news, width, missing in (([0], [40], 1, 2), ([16], [1], 1, 1), ([40, 3], [9, 60], 2, 3),
+                                           ([5, 0, 31], [30, 100, 1], 3, 4), ([64], [5], 2, 1)):
+        tables = torch.full((len(contexts), width), -1, dtype=torch.int32, device=device)
+        pages = iter(range(100, 200))
+        for b, c in enumerate(contexts):
+            for lp in range(min(width, -(-c // 16))):
+                tables[b, lp] = next(pages)
+        held = int((tables >= 0).sum())
+        p = serving.plan_step(ints(contexts), ints(news), tables, ints(list(range(20))), ints([20]),
+                              page_size=16, num_tokens=sum(news))
+        yield contexts, missing, held, tables.cpu(), p
+
+
+def check_narrow_table_plans(device):
+    for contexts, missing, held, tables, p in narrow_table_plans(device):
+        # every page that left the free list is in a table
+        assert int((tables >= 0).sum()) - held == 20 - int(p.free_count)
+        assert int(p.missing) == missing, contexts
+        starts, slots = p.q_starts.tolist(), p.slots.tolist()
+        for b, c in enumerate(contexts):
+            for row in range(starts[b], starts[b + 1]):
+                pos = c + row - starts[b]
+                page = int(tables[b, pos // 16]) if pos // 16 < tables.shape[1] else -1
+                assert slots[row] == (page * 16 + pos % 16 if page >= 0 else -1)
+
+
+def test_plan_keeps_the_pages_that_a_narrow_table_has_no_room_for():
+    check_narrow_table_plans("cpu")

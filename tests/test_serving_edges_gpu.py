@@ -178,3 +178,9 @@ def test_more_biases_than_the_kernel_takes_are_refused_before_the_first_step():
     assert lib().launch_count() == before
     most = LogitRules(bias={t: 100.0 for t in range(serving.MAX_BIAS)})
     assert max(generate_batch(art, model, ["a"], rules=most, **kw)[0].generated_token_ids) < serving.MAX_BIAS
+
+
+def test_plan_keeps_the_pages_that_a_narrow_table_has_no_room_for():
+    from test_batch_generation_edges import check_narrow_table_plans
+
+    check_narrow_table_plans(DEV)
