@@ -92,7 +92,8 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
 
 // One request as this kernel sees it.
 struct Request {
-  int q0, nq, kv, blocks, tiles;    // blocks of 8 * NT rows; tiles of one unit
+  // rows q0, q0 + 1, .. are positions ctx, ctx + 1, ..; the table holds the first kv positions
+  int q0, nq, ctx, kv, blocks, tiles;   // blocks of 8 * NT rows; tiles of one unit
   __device__ int64_t total(int Hkv) const { return static_cast<int64_t>(blocks) * Hkv * tiles; }
 };
 
@@ -101,7 +102,9 @@ __device__ __forceinline__ Request load_request(const Params& p, int b) {
   Request r;
   r.q0 = min(max(__ldg(p.q_starts + b), 0), p.T);
   r.nq = min(max(__ldg(p.q_starts + b + 1) - r.q0, 0), p.T - r.q0);
-  r.kv = min(max(__ldg(p.kv_lens + b), 0), p.width << p.page_shift);
+  const int len = max(__ldg(p.kv_lens + b), 0);
+  r.ctx = len - r.nq;
+  r.kv = min(len, p.width << p.page_shift);
   const int rows = r.nq <= p.max_rows / p.G ? r.nq * p.G : 0;
   r.blocks = (rows + 8 * NT - 1) / (8 * NT);
   r.tiles = max(1, (r.kv + kTile - 1) / kTile);
@@ -213,7 +216,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtasPerSm)
     const int per = (p.B + kThreads - 1) / kThreads;
     const int b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
     int64_t sum = 0;
-    Request r{0, 0, 0, 0, 1};
+    Request r{0, 0, 0, 0, 0, 1};
     for (int b = b0; b < b1; ++b) {
       r = load_request<NT>(p, b);
       sum += r.total(p.Hkv);
@@ -277,14 +280,15 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtasPerSm)
       s_found[1] = base;
       s_found[2] = r.q0;
       s_found[3] = r.nq;
-      s_found[4] = r.kv;
-      s_found[5] = r.blocks;
-      s_found[6] = r.tiles;
+      s_found[4] = r.ctx;
+      s_found[5] = r.kv;
+      s_found[6] = r.blocks;
+      s_found[7] = r.tiles;
     }
     __syncthreads();
     cur.b = s_found[0];
     cur.base = s_found[1];
-    cur.r = Request{s_found[2], s_found[3], s_found[4], s_found[5], s_found[6]};
+    cur.r = Request{s_found[2], s_found[3], s_found[4], s_found[5], s_found[6], s_found[7]};
     cur.set();
     __syncthreads();  // the merge area is free again
   }
@@ -410,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtasPerSm)
       // the row's largest magnitude goes to [2^14, 2^15) (fmaxf drops NaN; infinity stays)
       const int e = min(max(kv::exponent_of(amax) - 14, -100), 113);
       const float down = kv::pow2i(-e), up = kv::pow2i(e) * p.scale_log2;
-      const int see = live ? cur.r.kv - cur.r.nq + tok + 1 : 0;
+      const int see = live ? min(cur.r.ctx + tok + 1, cur.r.kv) : 0;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         row_scale[nt][i] = __shfl_sync(0xffffffffu, up, 8 * t4 + 4 * i);
@@ -440,7 +444,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtasPerSm)
         m_run[nt][i] = -INFINITY;
         l_run[nt][i] = 0.f;
       }
-    const int free_keys = cur.r.kv - cur.r.nq + rb * kRows / p.G + 1;  // keys that every row sees
+    const int free_keys = min(cur.r.ctx + rb * kRows / p.G + 1, cur.r.kv);  // keys that every row sees
 
 #pragma unroll 1
     for (int i = (warp - j0) & (kWarps - 1); i < cur.n; i += kWarps) {
@@ -659,7 +663,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtasPerSm)
       }
     const bool whole = cur.n == cur.r.tiles;
     // Keys that a token's rows see, and whether part of a row's numerator is large enough for them.
-    auto keys_of = [&](int tok) { return min(cur.r.kv, cur.r.kv - cur.r.nq + tok + 1); };
+    auto keys_of = [&](int tok) { return min(cur.r.kv, cur.r.ctx + tok + 1); };
     auto resolved = [&](const float4& x, float l, int tok) {
       const float top = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
       return top >= kResolved<INT8> * keys_of(tok) || !(l > 0.f && l < INFINITY);

@@ -207,10 +207,12 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const Params p) 
   }
   const int q0 = min(max(__ldg(p.q_starts + b), 0), p.T);
   const int n = min(max(__ldg(p.q_starts + b + 1) - q0, 0), p.T - q0);
-  const int kv = min(max(__ldg(p.kv_lens + b), 0), p.width << p.page_shift);
+  const int len = max(__ldg(p.kv_lens + b), 0);
+  const int ctx = len - n;                        // position of the first row
+  const int kv = min(len, p.width << p.page_shift);   // positions that the table holds
   const int tok0 = blk * 2 * tpt, toks = min(2 * tpt, n - tok0);
   // keys that the last row sees; the second row tile exists only if it has tokens
-  const int keys = max(0, min(kv, kv - n + tok0 + toks));
+  const int keys = max(0, min(kv, ctx + tok0 + toks));
   const int tiles = (keys + kPfKeys - 1) / kPfKeys;
   const int rts = toks > tpt ? 2 : 1;
 
@@ -378,7 +380,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const Params p) 
       publish(&k_full[st]);
       if (j + 1 < tiles) fetch(0, j + 1, page1);
       if (!wait_warp(&v_empty[st], ph ^ 1)) break;
-      if (!INT8 && (j + 1) * kPfKeys > kv - n + tok0 + 1) {
+      if (!INT8 && (j + 1) * kPfKeys > ctx + tok0 + 1) {
         // keys that some rows see and others do not: 0 * NaN would reach the others, so NaN
         // counts as 0 in the product and is put in at the end
         uint32_t bad = 0;
@@ -407,8 +409,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const Params p) 
     const uint32_t tO = tS - rt * 128 + 256 + rt * 128;
     const int tok = tok0 + rt * tpt + row / p.G, head = row % p.G;
     const bool live = row < tpt * p.G && tok < n;
-    const int limit = live ? kv - n + tok + 1 : 0;
-    const int first_limit = kv - n + tok0 + rt * tpt + 1;     // of the tile's first row
+    const int limit = live ? min(ctx + tok + 1, kv) : 0;
+    const int first_limit = min(ctx + tok0 + rt * tpt + 1, kv);     // of the tile's first row
     float row_scale = 0.f;
     if (rt < rts) {
       // this row's query, scaled to [2^14, 2^15) by a power of two, as f16
@@ -529,7 +531,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const Params p) 
       uint32_t nan_cols[D / 32] = {};
       if (!INT8 && tiles > 0 && *s_nan) {         // which columns of the keys this row sees
         const int* table = p.tables + b * p.table_stride;
-        for (int key = max(0, kv - n + tok0 + 1) / kPfKeys * kPfKeys; key < min(limit, kv); ++key) {
+        for (int key = max(0, ctx + tok0 + 1) / kPfKeys * kPfKeys; key < limit; ++key) {
           const int page = __ldg(table + (key >> p.page_shift));
           if (page < 0 || page >= p.num_pages) continue;
           const uint8_t* x = p.v_codes + (((static_cast<int64_t>(page) * p.Hkv + h) << p.page_shift) +
@@ -572,16 +574,15 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const Params p) 
         if (live && p.lse != nullptr)
           p.lse[at] = l_run == 0.f ? -INFINITY : m_run - kShift + log2f(l_run);
         // the last row first: if it sees no value but zeros, neither do the others
-        const int keys_seen = min(limit, kv);
         uint32_t again = __ballot_sync(0xffffffffu, l_run > 0.f && l_run < INFINITY &&
-                                                        top < kResolved<INT8> * keys_seen);
+                                                        top < kResolved<INT8> * limit);
 #pragma unroll 1
         while (again) {
           const int i = 31 - __clz(again);
           again ^= 1u << i;
           const int64_t row_at = __shfl_sync(0xffffffffu, at, i);
           const int64_t row_q = __shfl_sync(0xffffffffu, (q0 + tok) * p.q_row + (h * p.G + head) * p.q_head, i);
-          if (!exact_row<D, INT8>(p, b, h, p.q + row_q, __shfl_sync(0xffffffffu, keys_seen, i),
+          if (!exact_row<D, INT8>(p, b, h, p.q + row_q, __shfl_sync(0xffffffffu, limit, i),
                                   p.o + row_at * D, p.lse == nullptr ? nullptr : p.lse + row_at))
             break;
         }

@@ -211,7 +211,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, tables: torch.Tensor,
     positions; a row sees its own position and those before it. ``heads`` is a multiple of the
     cache's kv heads (grouped queries). ``max_new`` is an upper bound of the rows of one request.
     Rows past ``q_starts[B]`` and rows that see no key give 0; positions on a missing page
-    (table entry -1) are not seen. NaN in a position reaches the rows that see it and no others.
+    (table entry -1, or past the table's columns) are not seen. NaN in a position reaches the rows that see it and no others.
     ``lse`` (fp32 [tokens, heads]) receives the base-2 log-sum-exp of the scaled scores, -inf for
     rows that see nothing. Value scales of one request's pages may differ by up to 2**100.
 
@@ -236,6 +236,8 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, tables: torch.Tensor,
         r0, r1 = starts[b], starts[b + 1]
         if r1 <= r0 or n <= 0:
             continue
+        pos = n - (r1 - r0) + torch.arange(r1 - r0)
+        n = min(n, tables.shape[1] * ps)                     # positions past the table have no page
         ids = tables[b, :-(-n // ps)].long()
         there = ((ids >= 0) & (ids < cache.k_pages.shape[0])).repeat_interleave(ps)[:n]
         ids = ids.clamp(0, cache.k_pages.shape[0] - 1)
@@ -248,7 +250,6 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, tables: torch.Tensor,
 
         s = (q[r0:r1].to(cd).transpose(0, 1) @ dense(cache.k_pages, cache.k_scale).transpose(1, 2)
              ) * scale
-        pos = n - (r1 - r0) + torch.arange(r1 - r0)
         seen = (torch.arange(n)[None] <= pos[:, None]) & there[None]
         s = s.masked_fill(~seen, -math.inf)
         z = torch.logsumexp(s, -1)

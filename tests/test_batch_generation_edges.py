@@ -98,3 +98,36 @@ def check_narrow_table_plans(device):
 
 def test_plan_keeps_the_pages_that_a_narrow_table_has_no_room_for():
     check_narrow_table_plans("cpu")
+
+
+def lengths_beyond_the_table(device, D=64):
+    """(q, cache, narrow tables, wide tables, starts, lens): requests longer than their tables'
+    columns; the wide tables have the missing pages as -1."""
+    from nano_megatron_b200.ops import serving
+
+    def ints(v):
+        return torch.tensor(v, dtype=torch.int32, device=device)
+
+    g = torch.Generator().manual_seed(1)
+    cache = serving.PagedKV.create(12, 2, D, page_size=16, dtype=torch.int8, device=device)
+    k, v = (torch.randn(192, 2, D, generator=g).bfloat16().to(device) for _ in range(2))
+    serving.append_kv(cache, k, v, ints([[i, 16 * i, 0, 16] for i in range(12)]))
+    narrow = ints([[0, 1, 2], [3, 4, 5], [6, 7, 8], [9, 10, 11]])
+    wide = torch.cat([narrow, torch.full_like(narrow, -1)], 1)
+    lens, rows = [70, 49, 50, 96], [40, 1, 3, 60]      # 48 positions have a page
+    starts = [0, 40, 41, 44, 104]
+    q = torch.randn(104, 4, D, generator=g).bfloat16().to(device)
+    return q, cache, narrow, wide, ints(starts), ints(lens), rows
+
+
+def test_attention_sees_what_a_narrow_table_holds():
+    from nano_megatron_b200.ops import serving
+
+    q, cache, narrow, wide, starts, lens, rows = lengths_beyond_the_table("cpu")
+    got = [torch.empty(q.shape[:2]) for _ in range(2)]
+    a, b = (serving.paged_attention(q, cache, t, starts, lens, max_new=max(rows), lse=z)
+            for t, z in zip((narrow, wide), got))
+    # (another width may add up in another order: fp32 sums of 64 products of scores up to 8)
+    torch.testing.assert_close(a, b, rtol=2 ** -7, atol=2 ** -16)
+    torch.testing.assert_close(*got, rtol=0, atol=2 ** -16)
+    assert a.float().abs().amax((1, 2)).min() > 0

@@ -184,3 +184,22 @@ def test_plan_keeps_the_pages_that_a_narrow_table_has_no_room_for():
     from test_batch_generation_edges import check_narrow_table_plans
 
     check_narrow_table_plans(DEV)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("most", [1, 3, 60])
+def test_attention_sees_what_a_narrow_table_holds(D, most):
+    """Lengths past a table's columns are missing pages, not shorter requests: a row's position stays."""
+    from test_batch_generation_edges import lengths_beyond_the_table
+
+    q, cache, narrow, wide, starts, lens, rows = lengths_beyond_the_table(DEV, D)
+    pick = [i for i, r in enumerate(rows) if r <= most]
+    q = torch.cat([q[starts[i]:starts[i + 1]] for i in pick])
+    starts = [0]
+    for i in pick:
+        starts.append(starts[-1] + rows[i])
+    got = serving.paged_attention(q, cache, narrow[pick], ints(starts), lens[pick].contiguous(), max_new=most)
+    want, _ = _oracle(q, cache, wide[pick], starts, lens[pick].tolist(), D ** -0.5)
+    top = want.abs().amax(-1, keepdim=True)
+    assert float(top.min()) > 0
+    assert bool(((got.double() - want).abs() <= top * BOUND).all())
