@@ -54,12 +54,12 @@ __device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
 // One row of a request over its first `keys` positions by one warp, with fp32 probabilities and
 // without the value scales in the maximum: the plain formula. For the few rows that the f16
 // probabilities cannot resolve (see kResolved), so simple rather than fast: a lane per key for the
-// scores, a lane per D / 32 columns for the sum. Leaves a row alone, and returns false, if all the
-// values it sees are zero: 0 is right already. Pages' value scales may differ by up to 2^100
+// scores, a lane per D / 32 columns for the sum. With `look`, leaves a row alone, and returns false,
+// if all the values it sees are zero: its 0 is right already. Pages' value scales may differ by up to 2^100
 // (beyond, fp32 denominators lose keys that still count).
 template <int D, bool INT8>
 __device__ __forceinline__ bool exact_row(const Params& p, int b, int h, const __nv_bfloat16* q,
-                                          int keys, __nv_bfloat16* out, float* lse) {
+                                          int keys, bool look, __nv_bfloat16* out, float* lse) {
   constexpr int kCols = D / 32;
   const int lane = threadIdx.x & 31;
   const int* table = p.tables + b * p.table_stride;
@@ -69,7 +69,7 @@ __device__ __forceinline__ bool exact_row(const Params& p, int b, int h, const _
     if (page < 0 || page >= p.num_pages) return -1;
     return ((static_cast<int64_t>(page) * p.Hkv + h) << p.page_shift) + (key & (p.ps - 1));
   };
-  bool any = false;
+  bool any = !look;
 #pragma unroll 1
   for (int k0 = 0; k0 < keys && !any; k0 += 32) {
     const int64_t row = k0 + lane < keys ? row_of(k0 + lane) : -1;

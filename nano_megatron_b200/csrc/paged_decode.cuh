@@ -158,7 +158,8 @@ __device__ __forceinline__ int merge_at(int row, int u) {
   return row * 16 + (u ^ (D == 128 ? t : (t & 1) | ((t >> 1) << 2)));
 }
 
-// SEVERAL: requests may have several new tokens, so that a key can be hidden from some rows only.
+// SEVERAL: requests may have several new tokens, so that a key can be hidden from some rows only
+// (should one have several without it, its rows take the slow way of exact_row).
 template <int D, bool INT8, int NT, bool SEVERAL>
 __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtasPerSm)
     decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -664,7 +665,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtasPerSm)
     const bool whole = cur.n == cur.r.tiles;
     // Keys that a token's rows see, and whether part of a row's numerator is large enough for them.
     auto keys_of = [&](int tok) { return min(cur.r.kv, cur.r.ctx + tok + 1); };
+    // (without the NaN path, rows of a request of several are all done again: a `max_new` that is
+    // too small costs speed only)
+    const bool aside = !SEVERAL && cur.r.nq > 1;
     auto resolved = [&](const float4& x, float l, int tok) {
+      if (aside) return false;
       const float top = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
       return top >= kResolved<INT8> * keys_of(tok) || !(l > 0.f && l < INFINITY);
     };
@@ -822,7 +827,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtasPerSm)
         const int tok = (rb * kRows + row) / p.G, g = (rb * kRows + row) - tok * p.G;
         const int64_t at = static_cast<int64_t>(cur.r.q0 + tok) * p.Hq + h * p.G + g;
         exact_row<D, INT8>(p, cur.b, h, p.q + (cur.r.q0 + tok) * p.q_row + (h * p.G + g) * p.q_head,
-                           keys_of(tok), p.o + at * D, p.lse == nullptr ? nullptr : p.lse + at);
+                           keys_of(tok), !aside, p.o + at * D, p.lse == nullptr ? nullptr : p.lse + at);
       }
     }
   }

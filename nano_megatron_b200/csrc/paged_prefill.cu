@@ -582,7 +582,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const Params p) 
           again ^= 1u << i;
           const int64_t row_at = __shfl_sync(0xffffffffu, at, i);
           const int64_t row_q = __shfl_sync(0xffffffffu, (q0 + tok) * p.q_row + (h * p.G + head) * p.q_head, i);
-          if (!exact_row<D, INT8>(p, b, h, p.q + row_q, __shfl_sync(0xffffffffu, limit, i),
+          if (!exact_row<D, INT8>(p, b, h, p.q + row_q, __shfl_sync(0xffffffffu, limit, i), true,
                                   p.o + row_at * D, p.lse == nullptr ? nullptr : p.lse + row_at))
             break;
         }

@@ -209,7 +209,8 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, tables: torch.Tensor,
 
     Request ``b`` owns rows ``q_starts[b]:q_starts[b+1]``, the last of its ``kv_lens[b]`` cached
     positions; a row sees its own position and those before it. ``heads`` is a multiple of the
-    cache's kv heads (grouped queries). ``max_new`` is an upper bound of the rows of one request.
+    cache's kv heads (grouped queries). ``max_new`` is an upper bound of the rows of one request
+    (one that is too small costs speed only).
     Rows past ``q_starts[B]`` and rows that see no key give 0; positions on a missing page
     (table entry -1, or past the table's columns) are not seen. NaN in a position reaches the rows that see it and no others.
     ``lse`` (fp32 [tokens, heads]) receives the base-2 log-sum-exp of the scaled scores, -inf for

@@ -203,3 +203,25 @@ def test_attention_sees_what_a_narrow_table_holds(D, most):
     top = want.abs().amax(-1, keepdim=True)
     assert float(top.min()) > 0
     assert bool(((got.double() - want).abs() <= top * BOUND).all())
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("ctx", [0, 37, 3000])
+@pytest.mark.parametrize("zero", [False, True])
+def test_too_small_a_max_new_costs_speed_only(D, ctx, zero):
+    """Several rows although `max_new` says one: NaN still reaches only the rows that see it."""
+    from test_serving_ops_gpu import _filled
+
+    n = 4
+    cache, tables = _filled([ctx + n], 2, D, 16, E4M3)
+    if zero:
+        cache.v_pages.view(torch.uint8).zero_()
+    page, off = int(tables[0, (ctx + 2) // 16]), (ctx + 2) % 16
+    cache.v_pages.view(torch.uint8)[page, 0, off, 5] = 0xFF
+    cache.k_pages.view(torch.uint8)[page, 1, off, 3] = 0x7F
+    q = torch.randn(n, 8, D, device=DEV).bfloat16()
+    got, want = (serving.paged_attention(q, cache, tables, ints([0, n]), ints([ctx + n]), max_new=m)
+                 for m in (1, n))
+    assert torch.equal(got.isnan(), want.isnan()) and not bool(got[:2].isnan().any())
+    top = want.nan_to_num(0.0).double().abs().amax(-1, keepdim=True)
+    assert bool(((got.double() - want.double()).nan_to_num(0.0).abs() <= 2 * BOUND * top).all())
