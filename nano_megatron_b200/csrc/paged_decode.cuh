@@ -185,19 +185,24 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtasPerSm)
     return;
   }
 
-  // Rows past the last request's (padding) are zero; written at the end.
-  const int used = min(max(__ldg(p.q_starts + p.B), 0), p.T);
-  auto zero_padding = [&] {
+  // Rows before the first request's and past the last one's (padding) are zero; written at the end.
+  const bool padded = __ldg(p.q_starts) > 0 || __ldg(p.q_starts + p.B) < p.T;
+  auto zero_rows = [&](int from, int to) {
     constexpr int threads = kWarps * 32;
-    if (used >= p.T || tid >= threads) return;
-    const int64_t n = static_cast<int64_t>(p.T - used) * p.Hq * (D / 8);
-    uint4* o4 = reinterpret_cast<uint4*>(p.o) + static_cast<int64_t>(used) * p.Hq * (D / 8);
+    const int64_t n = static_cast<int64_t>(to - from) * p.Hq * (D / 8);
+    uint4* o4 = reinterpret_cast<uint4*>(p.o) + static_cast<int64_t>(from) * p.Hq * (D / 8);
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * threads + tid; i < n;
          i += static_cast<int64_t>(gridDim.x) * threads) {
       o4[i] = make_uint4(0, 0, 0, 0);
       if (p.lse != nullptr && i % (D / 8) == 0)
-        p.lse[static_cast<int64_t>(used) * p.Hq + i / (D / 8)] = -INFINITY;
+        p.lse[static_cast<int64_t>(from) * p.Hq + i / (D / 8)] = -INFINITY;
     }
+  };
+  auto zero_padding = [&] {
+    if (!padded || tid >= kWarps * 32) return;
+    const int first = min(max(__ldg(p.q_starts), 0), p.T);
+    zero_rows(0, first);
+    zero_rows(min(max(__ldg(p.q_starts + p.B), first), p.T), p.T);
   };
 
   // ---- this CTA's share of the tiles

@@ -211,7 +211,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, tables: torch.Tensor,
     positions; a row sees its own position and those before it. ``heads`` is a multiple of the
     cache's kv heads (grouped queries). ``max_new`` is an upper bound of the rows of one request
     (one that is too small costs speed only).
-    Rows past ``q_starts[B]`` and rows that see no key give 0; positions on a missing page
+    Rows before ``q_starts[0]`` or past ``q_starts[B]`` and rows that see no key give 0; positions on a missing page
     (table entry -1, or past the table's columns) are not seen. NaN in a position reaches the rows that see it and no others.
     ``lse`` (fp32 [tokens, heads]) receives the base-2 log-sum-exp of the scaled scores, -inf for
     rows that see nothing. Value scales of one request's pages may differ by up to 2**100.

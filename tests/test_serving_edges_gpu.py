@@ -225,3 +225,22 @@ def test_too_small_a_max_new_costs_speed_only(D, ctx, zero):
     assert torch.equal(got.isnan(), want.isnan()) and not bool(got[:2].isnan().any())
     top = want.nan_to_num(0.0).double().abs().amax(-1, keepdim=True)
     assert bool(((got.double() - want.double()).nan_to_num(0.0).abs() <= 2 * BOUND * top).all())
+
+
+@pytest.mark.parametrize("most", [2, 70])
+def test_rows_before_the_first_request_are_zero(most):
+    """A part of a plan: ``q_starts[1:]`` starts past row 0. Rows of nobody are 0, as on the CPU."""
+    cache = serving.PagedKV.create(8, 2, 64, page_size=32, dtype=INT8)
+    x = torch.randn(2 * most + 5, 3, 2, 64, device=DEV).bfloat16()
+    k, v, q = x.unbind(1)
+    tables = torch.full((3, 4), -1, dtype=torch.int32, device=DEV)
+    plan = serving.plan_step(ints([0, 0, 0]), ints([3, 2, 2 * most]), tables, ints(list(range(8))), ints([8]),
+                             page_size=32, num_tokens=2 * most + 5)
+    serving.append_kv(cache, k, v, plan.touched)
+    torch.full((64 << 20,), math.nan, device=DEV)        # what a new tensor would find in its memory
+    lse = torch.zeros(2 * most + 5, 2, device=DEV)
+    got = serving.paged_attention(q, cache, tables[1:], plan.q_starts[1:], plan.kv_lens[1:],
+                                  max_new=2 * most, lse=lse)
+    assert got[:3].abs().max() == 0 and bool((lse[:3] == -math.inf).all())
+    want = serving.paged_attention(q, cache, tables, plan.q_starts, plan.kv_lens, max_new=2 * most)
+    assert float(((got[3:] - want[3:]).abs().double() / want[3:].abs().amax(-1, keepdim=True)).max()) <= 2 * BOUND
