@@ -165,11 +165,6 @@ class BatchDecoder:
         tokens, context, fresh, rows = both.split([T, B, B, len(slots)])
         plan = serving.plan_step(context, fresh, self.tables, self.free_pages, self.free_count,
                                  page_size=self.page_size, num_tokens=T)
-        self.free_count = plan.free_count
-        self.free -= need
-        for s in slots:
-            self.lengths[s] += new[s]
-
         m = self.model
         h = m.embedding.weight.index_select(0, tokens)
         qc, kvc = self.nh * self.d, self.nkv * self.d
@@ -187,7 +182,13 @@ class BatchDecoder:
             gu = self._lin(y, w["wgu"], w["bgu"])
             h = h + self._lin(F.swiglu_act(gu, gu.shape[1] // 2), w["wd"], w["bd"])
         y, _ = F.rmsnorm(h.index_select(0, rows), m.final_norm.weight, self.eps)
-        return F.linear(y, m.lm_head.weight)[:, :m.original_vocab_size]
+        scores = F.linear(y, m.lm_head.weight)[:, :m.original_vocab_size]
+        # only now, so that a step that raised can be repeated
+        self.free_count = plan.free_count
+        self.free -= need
+        for s in slots:
+            self.lengths[s] += new[s]
+        return scores
 
 
 class _Rules:

@@ -131,3 +131,34 @@ def test_attention_sees_what_a_narrow_table_holds():
     torch.testing.assert_close(a, b, rtol=2 ** -7, atol=2 ** -16)
     torch.testing.assert_close(*got, rtol=0, atol=2 ** -16)
     assert a.float().abs().amax((1, 2)).min() > 0
+
+
+def test_a_step_that_fails_changes_nothing(tmp_path, monkeypatch):
+    """An error in the middle of the layers: lengths and pages stay, and the step can be repeated."""
+    from nano_megatron_b200.inference import BatchDecoder, batch
+
+    _, model = _artifact(tmp_path)
+    dec, other = (BatchDecoder(model, max_requests=2, max_len=64, page_size=16) for _ in range(2))
+    first, second = {0: list(range(5, 20))}, {0: [7, 8, 9], 1: list(range(30, 55))}
+    dec.step(first)
+    other.step(first)
+    before = _state(dec)
+    plain, calls = batch.F.swiglu_act, []
+
+    def failing(*a):
+        calls.append(1)
+        if len(calls) == 2:
+            raise RuntimeError("out of memory")
+        return plain(*a)
+
+    monkeypatch.setattr(batch.F, "swiglu_act", failing)
+    with pytest.raises(RuntimeError, match="out of memory"):
+        dec.step(second)
+    monkeypatch.setattr(batch.F, "swiglu_act", plain)
+    assert _state(dec) == before
+    assert torch.equal(dec.step(second), other.step(second))
+    assert _state(dec) == _state(other)
+    dec.release(0)
+    dec.release(1)
+    assert dec.free == int(dec.free_count) == dec.num_pages
+    assert sorted(dec.free_pages.tolist()) == list(range(dec.num_pages))
