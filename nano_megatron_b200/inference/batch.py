@@ -84,6 +84,8 @@ class BatchDecoder:
                  page_size: int = 64, cache_dtype: torch.dtype = torch.float8_e4m3fn) -> None:
         if max_requests < 1 or max_len < 1:
             raise ValueError("max_requests and max_len must be >= 1")
+        if page_size not in serving.PAGE_SIZES:
+            raise ValueError(f"page_size must be one of {serving.PAGE_SIZES}, got {page_size}")
         a0 = model.layers[0].attention
         self.model = model
         self.nh, self.nkv, self.d = a0.num_heads, a0.num_kv_heads, a0.head_dim

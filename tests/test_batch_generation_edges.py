@@ -162,3 +162,10 @@ def test_a_step_that_fails_changes_nothing(tmp_path, monkeypatch):
     dec.release(1)
     assert dec.free == int(dec.free_count) == dec.num_pages
     assert sorted(dec.free_pages.tolist()) == list(range(dec.num_pages))
+
+
+@pytest.mark.parametrize("page_size", [0, -16])
+def test_page_sizes_below_one_are_refused(tmp_path, page_size):
+    art, model = _artifact(tmp_path)
+    with pytest.raises(ValueError, match="page_size"):
+        _batch(art, model, page_size=page_size)
