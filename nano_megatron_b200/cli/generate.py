@@ -72,7 +72,9 @@ def run_generate(model: Path, prompt: str, *, device: str = "auto", dtype: str =
 def main(argv: Sequence[str] | None = None) -> None:
     a = parser().parse_args(argv)
     if a.prompts_file is not None:
-        prompts = a.prompts_file.read_text(encoding="utf-8").splitlines()
+        # (str.splitlines would also split at form feeds, line separators and others)
+        with open(a.prompts_file, encoding="utf-8") as f:
+            prompts = [line.removesuffix("\n") for line in f]
         for r in generate_batch_from_artifact(
                 a.model, prompts, device=a.device, dtype=a.dtype,
                 max_new_tokens=a.max_new_tokens, temperature=a.temperature, top_p=a.top_p,

@@ -169,3 +169,26 @@ def test_page_sizes_below_one_are_refused(tmp_path, page_size):
     art, model = _artifact(tmp_path)
     with pytest.raises(ValueError, match="page_size"):
         _batch(art, model, page_size=page_size)
+
+
+def _cli(tmp_path, monkeypatch, *args):
+    from nano_megatron_b200.cli import generate as gcli
+    from nano_megatron_b200.inference import batch
+
+    art, model = _artifact(tmp_path)
+    monkeypatch.setattr(batch, "load_model_for_generation", lambda *a, **k: (art, model, CPU))
+    gcli.main(["--model", "unused", "--max-new-tokens", "2", "--temperature", "0", *args])
+
+
+def test_prompts_file_is_split_at_line_ends_only(tmp_path, monkeypatch, capsys):
+    """Form feeds, separators and the like belong to a prompt: one result per line of the file."""
+    import json
+
+    lines = ["a\x0cb", "c d", "e\x1cf\x85g", "", "h"]
+    (tmp_path / "p.txt").write_bytes("\r\n".join(lines).encode())
+    _cli(tmp_path, monkeypatch, "--prompts-file", str(tmp_path / "p.txt"), "--json")
+    out = [json.loads(x) for x in capsys.readouterr().out.split("\n") if x]
+    assert [r["prompt"] for r in out] == lines
+    (tmp_path / "p.txt").write_text("a\nb\n\n")
+    _cli(tmp_path, monkeypatch, "--prompts-file", str(tmp_path / "p.txt"), "--json")
+    assert [json.loads(x)["prompt"] for x in capsys.readouterr().out.split("\n") if x] == ["a", "b", ""]
