@@ -43,16 +43,16 @@ def parser() -> argparse.ArgumentParser:
     p.add_argument("--kv-cache", action=argparse.BooleanOptionalAction, default=True,
                    help="reuse cached keys/values between decode steps (on by default; "
                         "--no-kv-cache recomputes the whole prefix every step)")
-    b = p.add_argument_group("batched generation (--prompts-file)")
-    b.add_argument("--max-batch", type=int, default=64, help="prompts served at a time")
-    b.add_argument("--cache-dtype", choices=("e4m3", "int8"), default="e4m3",
-                   help="8-bit format of the K/V cache")
-    b.add_argument("--repetition-penalty", type=float, default=1.0,
-                   help="divide positive scores of tokens seen before by this (1 = off)")
-    b.add_argument("--presence-penalty", type=float, default=0.0,
-                   help="subtract this from tokens that were generated before")
-    b.add_argument("--frequency-penalty", type=float, default=0.0,
-                   help="subtract this once per earlier generation of a token")
+    b = p.add_argument_group("batched generation (with --prompts-file only)")
+    b.add_argument("--max-batch", type=int, help="prompts served at a time (default: 64)")
+    b.add_argument("--cache-dtype", choices=("e4m3", "int8"),
+                   help="8-bit format of the K/V cache (default: e4m3)")
+    b.add_argument("--repetition-penalty", type=float,
+                   help="divide positive scores of tokens seen before by this (default: 1 = off)")
+    b.add_argument("--presence-penalty", type=float,
+                   help="subtract this from tokens that were generated before (default: 0)")
+    b.add_argument("--frequency-penalty", type=float,
+                   help="subtract this once per earlier generation of a token (default: 0)")
     p.add_argument("--json", action="store_true",
                    help="print the whole result (prompt, completion, token ids, stop reason) "
                         "as one JSON object instead of the text")
@@ -69,8 +69,26 @@ def run_generate(model: Path, prompt: str, *, device: str = "auto", dtype: str =
                                   use_kv_cache=kv_cache)
 
 
+# options of batched generation and their values when they are not given
+_BATCH_DEFAULTS = {"max_batch": 64, "cache_dtype": "e4m3", "repetition_penalty": 1.0,
+                   "presence_penalty": 0.0, "frequency_penalty": 0.0}
+
+
+def _check_mode(p: argparse.ArgumentParser, a: argparse.Namespace) -> None:
+    """Refuse options that the chosen mode would ignore; fill in the batch's defaults."""
+    for name, default in _BATCH_DEFAULTS.items():
+        if getattr(a, name) is None:
+            setattr(a, name, default)
+        elif a.prompts_file is None:
+            p.error(f"--{name.replace('_', '-')} needs --prompts-file")
+    if a.prompts_file is not None and not a.kv_cache:
+        p.error("--no-kv-cache: a batch is always served from its paged cache")
+
+
 def main(argv: Sequence[str] | None = None) -> None:
-    a = parser().parse_args(argv)
+    p = parser()
+    a = p.parse_args(argv)
+    _check_mode(p, a)
     if a.prompts_file is not None:
         # (str.splitlines would also split at form feeds, line separators and others)
         with open(a.prompts_file, encoding="utf-8") as f:

@@ -192,3 +192,33 @@ def test_prompts_file_is_split_at_line_ends_only(tmp_path, monkeypatch, capsys):
     (tmp_path / "p.txt").write_text("a\nb\n\n")
     _cli(tmp_path, monkeypatch, "--prompts-file", str(tmp_path / "p.txt"), "--json")
     assert [json.loads(x)["prompt"] for x in capsys.readouterr().out.split("\n") if x] == ["a", "b", ""]
+
+
+@pytest.mark.parametrize("option", [["--repetition-penalty", "1.2"], ["--presence-penalty", "0.5"],
+                                    ["--frequency-penalty", "0.5"], ["--cache-dtype", "int8"],
+                                    ["--max-batch", "2"]])
+def test_options_of_batches_are_refused_for_one_prompt(tmp_path, monkeypatch, capsys, option):
+    with pytest.raises(SystemExit):
+        _cli(tmp_path, monkeypatch, "--prompt", "x", *option)
+    assert option[0] in capsys.readouterr().err
+
+
+def test_recomputing_the_prefix_is_refused_for_batches(tmp_path, monkeypatch, capsys):
+    (tmp_path / "p.txt").write_text("a\n")
+    with pytest.raises(SystemExit):
+        _cli(tmp_path, monkeypatch, "--prompts-file", str(tmp_path / "p.txt"), "--no-kv-cache")
+    assert "--no-kv-cache" in capsys.readouterr().err
+    _cli(tmp_path, monkeypatch, "--prompts-file", str(tmp_path / "p.txt"), "--kv-cache")
+
+
+def test_options_of_batches_reach_them(tmp_path, monkeypatch):
+    from nano_megatron_b200.cli import generate as gcli
+
+    seen = {}
+    monkeypatch.setattr(gcli, "generate_batch_from_artifact", lambda *a, **k: seen.update(k) or [])
+    (tmp_path / "p.txt").write_text("a\n")
+    args = ["--model", "unused", "--prompts-file", str(tmp_path / "p.txt")]
+    gcli.main(args)
+    assert (seen["max_batch"], seen["cache_dtype"], seen["rules"].empty) == (64, "e4m3", True)
+    gcli.main(args + ["--max-batch", "3", "--cache-dtype", "int8", "--presence-penalty", "0.5"])
+    assert (seen["max_batch"], seen["cache_dtype"], seen["rules"].presence) == (3, "int8", 0.5)
