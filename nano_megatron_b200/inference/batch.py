@@ -93,6 +93,9 @@ class BatchDecoder:
         self.device = model.embedding.weight.device
         if self.device.type == "cuda" and self.d not in (64, 128):
             raise ValueError(f"batched generation on CUDA needs head_dim 64 or 128, not {self.d}")
+        if self.device.type == "cuda" and model.embedding.weight.dtype != torch.bfloat16:
+            raise ValueError("batched generation on CUDA needs bfloat16 weights, not "
+                             f"{model.embedding.weight.dtype}")
         self.max_requests, self.max_len, self.page_size = max_requests, max_len, page_size
         width = -(-max_len // page_size)
         self.num_pages = max_requests * width if num_pages is None else num_pages

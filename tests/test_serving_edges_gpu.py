@@ -244,3 +244,14 @@ def test_rows_before_the_first_request_are_zero(most):
     assert got[:3].abs().max() == 0 and bool((lse[:3] == -math.inf).all())
     want = serving.paged_attention(q, cache, tables, plan.q_starts, plan.kv_lens, max_new=2 * most)
     assert float(((got[3:] - want[3:]).abs().double() / want[3:].abs().amax(-1, keepdim=True)).max()) <= 2 * BOUND
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_weights_that_the_kernels_do_not_take_are_refused_at_once(dtype):
+    from test_batch_generation_gpu import _model
+
+    from nano_megatron_b200.inference import BatchDecoder
+
+    model, _ = _model(DEV, dtype, 4, 2)
+    with pytest.raises(ValueError, match="bfloat16"):
+        BatchDecoder(model, max_requests=1, max_len=16)
