@@ -25,6 +25,7 @@ from dataclasses import dataclass
 
 import torch
 
+from nano_megatron_b200.nn.rotary import rope_inv_freq
 from nano_megatron_b200.ops import functional as F
 
 from .artifact import InferenceArtifact, load_inference_artifact, local_parallel
@@ -159,7 +160,10 @@ class KVCacheDecoder:
         self.max_len = int(max_len)
         dev = model.embedding.weight.device
         dt = model.embedding.weight.dtype
-        self.inv_freq = model.rope_inv_freq.to(dev)
+        # The kernel takes fp32 frequencies, which a model cast to bf16 has rounded; on the CPU the
+        # model's own are used, as in its forward pass.
+        self.inv_freq = (rope_inv_freq(self.d, a0.rope_theta, device=dev) if dev.type == "cuda"
+                         else model.rope_inv_freq.to(dev))
         self.layers = [dict(w, k=torch.empty(self.max_len, self.nkv, self.d, device=dev, dtype=dt),
                             v=torch.empty(self.max_len, self.nkv, self.d, device=dev, dtype=dt))
                        for w in fused_layer_weights(model)]
