@@ -275,3 +275,23 @@ def test_single_prompt_decoding_of_bf16_weights():
         spread = (want - want.mean()).norm()
         for got in (single.forward(part), batch.step({0: part})[0]):
             assert float((got.float().cpu() - want).norm()) <= 0.06 * float(spread)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_repetition_at_the_ends_of_its_range(dtype):
+    """Scores of seen tokens: within 1.5 ulp of the quotient (one rounded reciprocal, one rounded
+    product) and 0.5 of the product, whatever the repetition."""
+    rep = torch.tensor([1.1, 1.3, 0.7, 3.0, 1e-39, 2.0 ** -126, 1e38, 3e38])
+    B, V = len(rep), 1000
+    z = torch.randn(B, V, generator=torch.Generator().manual_seed(0)).to(dtype)
+    z[4:6] *= 1e-3                                       # quotients within fp32
+    z[6:] *= 1e37
+    hist = torch.arange(V).expand(B, V).int().to(DEV)
+    got = serving.adjust_logits(z.to(DEV), hist, ints([V] * B), ints([V] * B), repetition=rep.to(DEV)).cpu()
+    f, r = z.double(), rep[:, None].double()
+    want = torch.where(f > 0, f / r, f * r)
+    over = want.abs() >= 2.0 ** 128
+    assert torch.equal(got.isinf(), over) and not bool(got.isnan().any())
+    got, want = got.masked_fill(over, 0.0), want.masked_fill(over, 0.0)
+    ulp = torch.exp2(torch.floor(torch.log2(want.abs().clamp(min=2.0 ** -126))) - 23)
+    assert bool(((got.double() - want).abs() <= torch.where(f > 0, 1.5, 0.5) * ulp).all())
