@@ -295,3 +295,89 @@ def test_repetition_at_the_ends_of_its_range(dtype):
     got, want = got.masked_fill(over, 0.0), want.masked_fill(over, 0.0)
     ulp = torch.exp2(torch.floor(torch.log2(want.abs().clamp(min=2.0 ** -126))) - 23)
     assert bool(((got.double() - want).abs() <= torch.where(f > 0, 1.5, 0.5) * ulp).all())
+
+
+@pytest.mark.parametrize("dtype", [E4M3, INT8])
+@pytest.mark.parametrize("D,Hq,H", [(64, 4, 4), (128, 8, 2)])
+@pytest.mark.parametrize("most", [1, 6, 150])
+def test_a_step_in_a_graph_follows_its_lengths(dtype, D, Hq, H, most):
+    """Plan, cache write, read, attention and logit rules captured once and replayed with other
+    lengths, rows and histories: as the same calls made one by one."""
+    B, page, V, T = 5, 32, 3000, 5 * most
+    g = torch.Generator().manual_seed(most)
+
+    def make(seed):
+        cache = _cache(200, H, D, page, dtype)
+        tables = torch.full((B, 30), -1, dtype=torch.int32, device=DEV)
+        order = torch.randperm(200, generator=torch.Generator().manual_seed(seed)).int().to(DEV)
+        return cache, tables, order, ints([200])
+
+    context, new = ints([0] * B), ints([0] * B)
+    q, k, v = (torch.zeros(T, h, D, device=DEV, dtype=torch.bfloat16) for h in (Hq, H, H))
+    logits, history = torch.zeros(B, V, device=DEV), torch.zeros(B, 700, dtype=torch.int32, device=DEV)
+    prompts, rep = ints([3] * B), torch.full((B,), 1.2, device=DEV)
+
+    def step(cache, tables, free, count):
+        p = serving.plan_step(context, new, tables, free, count, page_size=page, num_tokens=T)
+        serving.append_kv(cache, k, v, p.touched)
+        o = serving.paged_attention(q, cache, tables, p.q_starts, p.kv_lens, max_new=most)
+        z = serving.adjust_logits(logits, history, p.kv_lens, prompts, repetition=rep, presence=rep)
+        return (o, z, *serving.read_kv(cache, p.slots), *p)
+
+    graphed, eager = make(1), make(1)
+    spare = make(2)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*spare)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(*graphed)
+    lens = [0] * B
+    for turn in range(4):
+        adds = [int(torch.randint(1 if turn else 0, most + 1, (1,), generator=g)) for _ in range(B)]
+        adds[turn % B] = most
+        context.copy_(ints(lens))
+        new.copy_(ints(adds))
+        for t in (q, k, v):
+            t.copy_(torch.randn(t.shape, generator=g))
+        logits.copy_(torch.randn(B, V, generator=g))
+        history.copy_(torch.randint(0, V, (B, 700), generator=g))
+        graph.replay()
+        want = step(*eager)
+        for a, b in zip(out, want):
+            assert torch.equal(a.nan_to_num(3.0) if a.is_floating_point() else a,
+                               b.nan_to_num(3.0) if b.is_floating_point() else b)
+        for a, b in zip((*graphed[0], graphed[1]), (*eager[0], eager[1])):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+        for case in (graphed, eager):
+            case[3].copy_(want[-2])                      # free_count
+        lens = [a + b for a, b in zip(lens, adds)]
+    check_status(torch.device(DEV))
+
+
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 1e-6])
+@pytest.mark.parametrize("contexts,news", [([100, 37], [1, 1]), ([100, 37], [5, 3]), ([300, 200], [200, 90])])
+@pytest.mark.parametrize("dtype", [E4M3, INT8])
+def test_softmax_scales_of_zero_and_below(scale, contexts, news, dtype):
+    from test_serving_ops_gpu import _filled
+
+    cache, tables = _filled(contexts, 2, 64, 16, dtype)
+    starts = [0, news[0], sum(news)]
+    q = torch.randn(sum(news), 8, 64, device=DEV).bfloat16()
+    got = serving.paged_attention(q, cache, tables, ints(starts), ints(contexts), max_new=max(news),
+                                  softmax_scale=scale)
+    want, _ = _oracle(q, cache, tables, starts, contexts, scale)
+    top = want.abs().amax(-1, keepdim=True)
+    assert bool(((got.double() - want).abs() <= top * BOUND).all())
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("G", [48, 65, 96, 128, 129, 200])
+@pytest.mark.parametrize("new", [1, 3])
+def test_wide_groups(D, G, new):
+    """More heads of a group than a prompt's row tile halves, fills, and holds."""
+    from test_serving_ops_gpu import _check
+
+    _check([150, 33, 64], [new, 1, new], 2 * G, 2, D, 32, E4M3)
