@@ -268,6 +268,8 @@ def generate_batch(artifact: InferenceArtifact, model, prompts: Sequence[str], *
     largest length needed): a waiting prompt is admitted when a slot and pages for its whole
     length are free.
     """
+    if isinstance(prompts, str):
+        raise TypeError("prompts must be a list of texts, not one text")
     prompts = list(prompts)
     for p in prompts:
         _check_args(p, max_new_tokens, temperature, top_p, top_k, seed, add_bos)

@@ -222,3 +222,9 @@ def test_options_of_batches_reach_them(tmp_path, monkeypatch):
     assert (seen["max_batch"], seen["cache_dtype"], seen["rules"].empty) == (64, "e4m3", True)
     gcli.main(args + ["--max-batch", "3", "--cache-dtype", "int8", "--presence-penalty", "0.5"])
     assert (seen["max_batch"], seen["cache_dtype"], seen["rules"].presence) == (3, "int8", 0.5)
+
+
+def test_a_text_is_not_a_list_of_prompts(tmp_path):
+    art, model = _artifact(tmp_path)
+    with pytest.raises(TypeError, match="prompts"):
+        _batch(art, model, "once upon")
