@@ -96,6 +96,9 @@ class BatchDecoder:
         if self.device.type == "cuda" and model.embedding.weight.dtype != torch.bfloat16:
             raise ValueError("batched generation on CUDA needs bfloat16 weights, not "
                              f"{model.embedding.weight.dtype}")
+        if self.device.type == "cuda" and max_requests > serving.MAX_REQUESTS:
+            raise ValueError(f"at most {serving.MAX_REQUESTS} requests at a time on CUDA, "
+                             f"got {max_requests}")
         self.max_requests, self.max_len, self.page_size = max_requests, max_len, page_size
         width = -(-max_len // page_size)
         self.num_pages = max_requests * width if num_pages is None else num_pages

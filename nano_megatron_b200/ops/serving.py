@@ -32,6 +32,7 @@ from ._ext import lib, status_word
 
 PAGE_SIZES = (16, 32, 64, 128)
 CODE_TYPES = {torch.float8_e4m3fn: 448.0, torch.int8: 127.0}
+MAX_REQUESTS = 4096           # requests of a step that the kernel of ``plan_step`` takes
 MAX_BIAS = 1024               # biases of a row that the kernel of ``adjust_logits`` takes
 _SCALE_EXP = 60
 
@@ -93,7 +94,7 @@ def plan_step(context_lens: torch.Tensor, new_lens: torch.Tensor, tables: torch.
     ``tables`` [>= B, P] holds each request's pages; entries for the pages that the new tokens
     open are written here, taken from the end of ``free_pages[:free_count]`` in request order.
     ``num_tokens`` is the number of rows the step has (the sum of ``new_lens``, or more when the
-    rest is padding; rows beyond it are dropped). ``free_count`` is not changed: the plan's own
+    rest is padding; rows beyond it are dropped). On CUDA a step has at most ``MAX_REQUESTS``. ``free_count`` is not changed: the plan's own
     ``free_count`` is what is left.
     """
     if context_lens.is_cuda:
@@ -162,7 +163,7 @@ def _encode(x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
 def append_kv(cache: PagedKV, k: torch.Tensor, v: torch.Tensor, touched: torch.Tensor) -> None:
     """Write rows ``k`` / ``v`` [tokens, kv_heads, head_dim] into the pages that a plan's
     ``touched`` lists. A page whose scale grows has its older codes rescaled; a page written
-    from offset 0 starts anew."""
+    from offset 0 starts anew. ``touched`` lists a page once, as a plan does."""
     if cache.k_pages.is_cuda:
         lib().append_kv(*cache, k, v, touched)
         return

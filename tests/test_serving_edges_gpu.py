@@ -381,3 +381,15 @@ def test_wide_groups(D, G, new):
     from test_serving_ops_gpu import _check
 
     _check([150, 33, 64], [new, 1, new], 2 * G, 2, D, 32, E4M3)
+
+
+def test_more_requests_than_a_plan_takes_are_refused_at_once():
+    from test_batch_generation_gpu import _model
+
+    from nano_megatron_b200.inference import BatchDecoder
+
+    model, _ = _model(DEV, torch.bfloat16, 4, 2)
+    with pytest.raises(ValueError, match=str(serving.MAX_REQUESTS)):
+        BatchDecoder(model, max_requests=serving.MAX_REQUESTS + 1, max_len=16, num_pages=1)
+    dec = BatchDecoder(model, max_requests=serving.MAX_REQUESTS, max_len=16, page_size=16, num_pages=1)
+    assert bool(dec.step({serving.MAX_REQUESTS - 1: [5]}).isfinite().all())
