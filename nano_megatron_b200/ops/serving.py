@@ -94,8 +94,8 @@ def plan_step(context_lens: torch.Tensor, new_lens: torch.Tensor, tables: torch.
     ``tables`` [>= B, P] holds each request's pages; entries for the pages that the new tokens
     open are written here, taken from the end of ``free_pages[:free_count]`` in request order.
     ``num_tokens`` is the number of rows the step has (the sum of ``new_lens``, or more when the
-    rest is padding; rows beyond it are dropped). On CUDA a step has at most ``MAX_REQUESTS``. ``free_count`` is not changed: the plan's own
-    ``free_count`` is what is left.
+    rest is padding; rows beyond it are dropped). ``free_count`` is not changed: the plan's own
+    ``free_count`` is what is left. On CUDA a step has at most ``MAX_REQUESTS``.
     """
     if context_lens.is_cuda:
         return StepPlan._make(lib().plan_step(context_lens, new_lens, tables, free_pages,
