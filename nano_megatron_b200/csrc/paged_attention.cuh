@@ -7,17 +7,18 @@ namespace nmb {
 namespace paged {
 
 // Probabilities in f16. A row's running maximum M of t = score + log2 of the value scale moves when
-// a tile exceeds it by 2^4 (most tiles then skip rescaling the accumulator), and probabilities are
-// stored as 2^(t - M + 11): at most 2^15, with all 11 bits down to 2^-25 of 2^M and a quantum of
+// a tile exceeds it by 2^6 (most tiles then skip rescaling the accumulator; prompts of up to 2048
+// tokens over as many, 32 / 8 heads of 128: 239.6 us with 2^4, 235.2 with 2^8), and probabilities are
+// stored as 2^(t - M + 9): at most 2^15, with all 11 bits down to 2^-23 of 2^M and a quantum of
 // 2^-24 (error 2^-25) below that.
-constexpr float kLazy = 4.f;
-constexpr float kShift = 11.f;
+constexpr float kLazy = 6.f;
+constexpr float kShift = 9.f;
 
 // That error of a key's probability matters only where the whole result is small: where M comes
 // from a key whose own value is next to nothing, because its page's scale was raised by another
 // key or because it just takes the weight. A row whose largest numerator is at least this times its
 // keys is within 2^-11 of it (keys * largest code * 2^-25); the others are computed again by
-// exact_row. A key with a code of 8 at the maximum is enough for 600,000 keys.
+// exact_row. A key with a code of 8 at the maximum is enough for 149,000 keys.
 template <bool INT8>
 constexpr float kResolved = (INT8 ? 127.f : 448.f) / 16384.f;
 

@@ -71,7 +71,7 @@ struct Cfg {
   static constexpr int kRing = kStages * kStageBytes;
   static constexpr int kMerge = kWarps * 8 * 64 * 4;        // 8 rows by 64 columns at a time
   static constexpr int kStats = (kWarps + 1) * 8 * NT * 8;
-  static constexpr int kSmem = kRing + kMerge + kStats + kStages * 16 + kStages * 16 + 16 + 8 * NT * 4;
+  static constexpr int kSmem = kRing + kMerge + kStats + kStages * 16 + kStages * 16 + 16;
 };
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
@@ -158,12 +158,23 @@ __device__ __forceinline__ int merge_at(int row, int u) {
   return row * 16 + (u ^ (D == 128 ? t : (t & 1) | ((t >> 1) << 2)));
 }
 
+// exact_row in a function of its own: inlined, it took registers and instruction cache from the
+// kernels that hardly ever need it (19 requests of 35 tokens, 8 heads of 128: 16.2 us, 14.4 with the call).
+template <int D, bool INT8>
+__device__ __noinline__ void exact_row_aside(const Params& p, int b, int q0, int ctx, int kv, int h, int row,
+                                             bool look) {
+  const int tok = row / p.G, head = h * p.G + row - tok * p.G;
+  const int64_t at = static_cast<int64_t>(q0 + tok) * p.Hq + head;
+  exact_row<D, INT8>(p, b, h, p.q + (q0 + tok) * p.q_row + head * p.q_head, min(kv, ctx + tok + 1), look,
+                     p.o + at * D, p.lse == nullptr ? nullptr : p.lse + at);
+}
+
 // SEVERAL: requests may have several new tokens, so that a key can be hidden from some rows only
 // (should one have several without it, its rows take the slow way of exact_row).
 template <int D, bool INT8, int NT, bool SEVERAL>
 __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtasPerSm)
     decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                  const Params p) {
+                  const __grid_constant__ Params p) {
   using C = Cfg<D, NT>;
   constexpr int S = C::kStages;
   constexpr int kSteps = D / 16;
@@ -177,7 +188,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtasPerSm)
   uint64_t* full = reinterpret_cast<uint64_t*>(s_info + S);
   uint64_t* empty = full + S;
   volatile int* s_flag = reinterpret_cast<volatile int*>(empty + S);         // abort, last
-  volatile int* s_ok = s_flag + 4;                                           // [row] see kResolved
 
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid / 32, 0);
   if (smem_u32(smem) & 1023u) {     // the swizzle pattern needs 1024-byte alignment
@@ -662,25 +672,23 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtasPerSm)
           l = fmaf(st.y, ex2(st.x - ref), l);
         }
         corr[nt][c] = ex2(m_run[nt][c] - ref);
-        if (warp == 0 && g8 == 0) {
-          s_tot[row] = make_float2(m, l);
-          s_ok[row] = 0;
-        }
+        if (warp == 0 && g8 == 0) s_tot[row] = make_float2(m, l);
       }
     const bool whole = cur.n == cur.r.tiles;
-    // Keys that a token's rows see, and whether part of a row's numerator is large enough for them.
-    auto keys_of = [&](int tok) { return min(cur.r.kv, cur.r.ctx + tok + 1); };
-    // (without the NaN path, rows of a request of several are all done again: a `max_new` that is
-    // too small costs speed only)
-    const bool aside = !SEVERAL && cur.r.nq > 1;
-    auto resolved = [&](const float4& x, float l, int tok) {
-      if (aside) return false;
-      const float top = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
-      return top >= kResolved<INT8> * keys_of(tok) || !(l > 0.f && l < INFINITY);
+    // A row is computed again unless one of its numerators reaches this. (kv bounds the keys it sees.
+    // Without the NaN path, all rows of a request of several are: a `max_new` that is too small costs
+    // speed only.)
+    const float enough = !SEVERAL && cur.r.nq > 1 ? INFINITY : kResolved<INT8> * cur.r.kv;
+    auto again = [&](int row) {
+      exact_row_aside<D, INT8>(p, cur.b, cur.r.q0, cur.r.ctx, cur.r.kv, h, rb * kRows + row,
+                               SEVERAL || cur.r.nq == 1);
     };
     const int slot = blockIdx.x * 2 + (first_run ? 0 : 1);
     float* part = p.part + static_cast<int64_t>(slot) * (kRows * D);
     constexpr int kParts = D / 64;  // 64 columns at a time; at D = 128 those of even, then odd g8
+    static_assert(kWarps * 32 == 8 * 16, "16 lanes a row, the same ones in every part");
+    float top = 0.f;                // of this thread's columns of its row
+    uint32_t redo = 0;              // bit 2 * nt + i: row 8 * nt + 2 * warp + i
 #pragma unroll
     for (int np = 0; np < NT * kParts; ++np) {
       const int nt = np / kParts, part_cols = np % kParts;
@@ -699,12 +707,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtasPerSm)
       }
       sync_all();
       const int in = min(8, rows - nt * 8);
-      for (int u = tid; u < in * 16; u += kWarps * 32) {
-        const int r8 = u / 16, q = part_cols * 16 + u % 16, row = nt * 8 + r8;
+      const int r8 = tid / 16, q = part_cols * 16 + tid % 16, row = nt * 8 + r8;
+      if (part_cols == 0) top = r8 < in ? 0.f : INFINITY;
+      if (r8 < in) {
         float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-          const float4 y = s_merge[w * 8 * 16 + merge_at<D>(r8, u % 16)];
+          const float4 y = s_merge[w * 8 * 16 + merge_at<D>(r8, tid % 16)];
           x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
         }
         const float2 tot = s_tot[row];
@@ -714,7 +723,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtasPerSm)
           const int64_t at = static_cast<int64_t>(cur.r.q0 + tok) * p.Hq + head;
           *reinterpret_cast<uint2*>(p.o + at * D + q * 4) =
               make_uint2(pack_bf16x2(x.x * inv, x.y * inv), pack_bf16x2(x.z * inv, x.w * inv));
-          if (resolved(x, tot.y, tok)) s_ok[row] = 1;
+          top = fmaxf(top, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
           if (p.lse != nullptr && q == 0)
             p.lse[at] = tot.y == 0.f ? -INFINITY : tot.x - kShift + log2f(tot.y);
         } else {
@@ -722,11 +731,24 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtasPerSm)
           if (q == 0) p.part_ml[slot * kRows + row] = tot;
         }
       }
+      if (part_cols == kParts - 1) {
+        const uint32_t fine = __ballot_sync(0xffffffffu, top >= enough);
+        redo |= ((fine & 0xffffu ? 0u : 1u) | (fine >> 16 ? 0u : 2u)) << (2 * nt);
+      }
     }
+    if (whole) {
+#pragma unroll 1
+      for (; __builtin_expect(redo != 0, 0); redo &= redo - 1) {
+        const int i = __ffs(redo) - 1;
+        again(i / 2 * 8 + 2 * warp + (i & 1));
+      }
+      continue;
+    }
+
     // ---- a unit shared with other CTAs: the last to finish adds the parts up in CTA order
     sync_all();
     const int rpt = (p.G + kRows - 1) / kRows;
-    if (tid == 0 && !whole) {
+    if (tid == 0) {
       int* counter = p.counters + (static_cast<int64_t>(h) * p.T + cur.r.q0) * rpt + rb;
       __threadfence();              // the barrier and this fence publish the whole CTA's part
       const int before = atomicAdd(counter, cur.n);
@@ -735,8 +757,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtasPerSm)
       __threadfence();
       s_flag[1] = last;
     }
-    if (!whole) sync_all();
-    if (!whole && s_flag[1]) {
+    sync_all();
+    if (s_flag[1]) {
       const int u0 = cur.base + cur.unit * cur.r.tiles, u1 = u0 + cur.r.tiles;
       auto owner = [&](int tile) {
         const int group = tile / span, longer = extra * (share + 1), t = tile - group * span;
@@ -820,19 +842,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtasPerSm)
         if (odd == 0)
           *reinterpret_cast<uint2*>(p.o + at * D + col) =
               make_uint2(pack_bf16x2(x.x * inv, x.y * inv), pack_bf16x2(x.z * inv, x.w * inv));
-        if (resolved(x, l, tok)) s_ok[row] = 1;
         if (p.lse != nullptr && lane == 0) p.lse[at] = l == 0.f ? -INFINITY : m - kShift + log2f(l);
-      }
-      sync_all();
-    }
-    if (whole || s_flag[1]) {
-#pragma unroll 1
-      for (int row = warp; row < rows; row += kWarps) {
-        if (s_ok[row]) continue;
-        const int tok = (rb * kRows + row) / p.G, g = (rb * kRows + row) - tok * p.G;
-        const int64_t at = static_cast<int64_t>(cur.r.q0 + tok) * p.Hq + h * p.G + g;
-        exact_row<D, INT8>(p, cur.b, h, p.q + (cur.r.q0 + tok) * p.q_row + (h * p.G + g) * p.q_head,
-                           keys_of(tok), !aside, p.o + at * D, p.lse == nullptr ? nullptr : p.lse + at);
+        const float top = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+        if (!__any_sync(0xffffffffu, top >= enough)) again(row);
       }
     }
   }

@@ -12,7 +12,7 @@
 // share every converted key) of one request and kv head, 512 threads:
 //   warps 0-3, 4-7 : softmax of tile 0 / 1, a thread per row: loads S (tcgen05.ld), online softmax
 //                    in base 2, writes P (f16) over S in TMEM, rescales O there when the maximum
-//                    grows by more than 2^4, and stores the result at the end;
+//                    grows by more than 2^6, and stores the result at the end;
 //   warps 8-11     : converters: cache codes from global memory (prefetched into registers one
 //                    tile ahead) to f16 tiles in shared memory, in the K-major / MN-major
 //                    128-byte-swizzled layouts that tcgen05.mma reads, two stages each of K and V;
