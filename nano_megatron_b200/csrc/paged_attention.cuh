@@ -128,7 +128,7 @@ __device__ __forceinline__ bool exact_row(const Params& p, int b, int h, const _
       }
     }
   }
-  const float inv = 1.f / l;
+  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;   // a row that sees nothing: 0
   __syncwarp();                       // what this warp wrote there before
 #pragma unroll
   for (int i = 0; i < kCols; i += 2)

@@ -393,3 +393,18 @@ def test_more_requests_than_a_plan_takes_are_refused_at_once():
         BatchDecoder(model, max_requests=serving.MAX_REQUESTS + 1, max_len=16, num_pages=1)
     dec = BatchDecoder(model, max_requests=serving.MAX_REQUESTS, max_len=16, page_size=16, num_pages=1)
     assert bool(dec.step({serving.MAX_REQUESTS - 1: [5]}).isfinite().all())
+
+
+def test_rows_without_keys_and_too_small_a_max_new():
+    """Rows that see nothing among several of a request, although `max_new` says one: 0, not NaN."""
+    cache = serving.PagedKV.create(4, 1, 64, page_size=16)
+    x = torch.randn(20, 2, 1, 64, device=DEV).bfloat16()
+    serving.append_kv(cache, x[:, 0], x[:, 1], ints([[0, 0, 0, 16], [1, 16, 0, 4]]))
+    q = torch.randn(6, 2, 64, device=DEV).bfloat16()
+    for tables, lens, hidden in (([[0, 1]], [4], 2), ([[-1, 1]], [20], 1), ([[-1, -1]], [20], 6)):
+        lse = torch.zeros(6, 2, device=DEV)
+        got = serving.paged_attention(q, cache, ints(tables), ints([0, 6]), ints(lens), max_new=1, lse=lse)
+        assert got[:hidden].abs().max() == 0 and bool((lse[:hidden] == -math.inf).all())
+        want, _ = _oracle(q, cache, ints(tables), [0, 6], lens, 0.125)
+        top = want.abs().amax(-1, keepdim=True)
+        assert bool(((got.double() - want).abs() <= top * BOUND).all())
