@@ -12,8 +12,8 @@
 // 2^-39 of it. Sums are fp32.
 //
 // Decode kernel (few query rows per request: decoding, short continuations). Bound by reading
-// the codes of K and V once: 128 requests of 512 to 4096 tokens, 8 kv heads of 128, take 123 us, 5.6 TB/s
-// or 86 % of the measured copy rate.
+// the codes of K and V once: 128 requests of 512 to 4096 tokens, 8 kv heads of 128, take 121 us, 5.7 TB/s
+// or 87 % of the measured copy rate.
 //  * A unit is (request, kv head, block of 8 or 16 query rows = tokens x heads of the group). Its
 //    keys are cut into tiles of 32; the tiles of all units, in order, are dealt evenly to the
 //    CTAs, whatever the lengths (every CTA scans the B lengths for itself). A unit that is shared
