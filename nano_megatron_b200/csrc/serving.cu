@@ -389,8 +389,6 @@ __global__ void __launch_bounds__(kLogitThreads) logits_kernel(const LogitParams
     reinterpret_cast<int4*>(s_count)[i] = make_int4(0, 0, 0, 0);
   const int len = min(max(p.lens[row], 0), p.L), prompt = p.prompts[row];
   const float rep = p.repetition ? p.repetition[row] : 1.f;
-  int rep_exp;
-  const float rep_part = frexpf(rep, &rep_exp);   // [0.5, 1)
   const float pre = p.presence ? p.presence[row] : 0.f, freq = p.frequency ? p.frequency[row] : 0.f;
   const T* z = static_cast<const T*>(p.logits) + row * p.stride + v0;
   float* o = p.out + row * p.out_stride + v0;
@@ -419,11 +417,10 @@ __global__ void __launch_bounds__(kLogitThreads) logits_kernel(const LogitParams
   }
   __syncthreads();
   // One reciprocal a row: x * (1 / rep) is within 1.5 ulp of x / rep and an eighth of its work (128
-  // rows of 32768: 12.0 us a call, 13.1 with divisions). In two factors, neither of which leaves
-  // fp32's normal range however large or small the repetition is.
-  const float inv = ldexpf(1.f / rep_part, -rep_exp / 2), inv2 = ldexpf(1.f, -rep_exp - -rep_exp / 2);
+  // rows of 32768: 12.0 us a call, 13.1 with divisions).
+  const float inv = 1.f / rep;
   auto rule = [&](float x, int count) {
-    if (count != 0) x = x > 0.f ? x * inv * inv2 : x * rep;
+    if (count != 0) x *= x > 0.f ? inv : rep;
     count &= ~kSeen;
     return count > 0 ? x - freq * count - pre : x;
   };
@@ -450,6 +447,16 @@ __global__ void __launch_bounds__(kLogitThreads) logits_kernel(const LogitParams
     } else {
       for (int e = 0; e < 8 && c + e < n; ++e)
         o[c + e] = (bits >> e) & 1u ? rule(to_float(z[c + e]), s_count[c + e]) : -INFINITY;
+    }
+  }
+  if (!(rep >= 0x1p-126f && rep <= 0x1p126f)) {  // not a normal reciprocal: the same with divisions
+    __syncthreads();
+    for (int t = threadIdx.x; t < n; t += kLogitThreads) {
+      const int seen = s_count[t], count = seen & ~kSeen;
+      if (seen == 0 || (allowed && !((allowed[(v0 + t) >> 5] >> ((v0 + t) & 31)) & 1))) continue;
+      float x = to_float(z[t]);
+      x = x > 0.f ? x / rep : x * rep;
+      o[t] = count > 0 ? x - freq * count - pre : x;
     }
   }
   if (p.NB == 0) return;

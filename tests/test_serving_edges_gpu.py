@@ -408,3 +408,30 @@ def test_rows_without_keys_and_too_small_a_max_new():
         want, _ = _oracle(q, cache, ints(tables), [0, 6], lens, 0.125)
         top = want.abs().amax(-1, keepdim=True)
         assert bool(((got.double() - want).abs() <= top * BOUND).all())
+
+
+@pytest.mark.parametrize("rep", [2e-39, 2.0 ** 127])
+@pytest.mark.parametrize("V", [700, 20001])
+def test_all_rules_with_a_repetition_out_of_the_normal_range(rep, V):
+    """The other rules around it: penalties, mask, biases, tokens that do not occur."""
+    from test_serving_ops_gpu import _logits_oracle
+
+    g = torch.Generator().manual_seed(V)
+    z = torch.randn(2, V, generator=g) * (1e-2 if rep < 1 else 1.0)
+    hist = torch.randint(0, V, (2, 300), generator=g).int()
+    lens, prompts = [300, 100], [150, 0]
+    rep, pre, freq = torch.full((2,), rep), torch.tensor([0.3, 0.1]), torch.tensor([0.0, 0.2])
+    z = torch.where((torch.rand(2, V, generator=g) < 0.5) | (rep[:, None] < 1), z, z * 1e-30)
+    z[z < 0] *= 1e-10                                     # products within fp32
+    ids, bias = torch.randint(0, V, (2, 9), generator=g).int(), torch.randn(2, 9, generator=g)
+    ids[:, :4] = hist[:, :4]
+    allowed = torch.randint(-2 ** 31, 2 ** 31 - 1, (2, (V + 31) // 32), generator=g).int()
+    got = serving.adjust_logits(z.to(DEV), hist.to(DEV), ints(lens), ints(prompts),
+                                **{k: t.to(DEV) for k, t in dict(repetition=rep, presence=pre, frequency=freq,
+                                                                 bias_ids=ids, bias=bias, allowed=allowed).items()}).cpu()
+    want = _logits_oracle(z, hist, lens, prompts, rep, pre, freq, ids, bias, allowed)
+    assert torch.equal(torch.isinf(got), torch.isinf(want))
+    ok = ~torch.isinf(want)
+    # a quotient or product, up to two penalties and a few biases: an ulp or so of the largest of them each
+    err, size = (got.double() - want)[ok].abs(), want[ok].abs() + 16.0
+    assert bool((err <= 4 * size * 2.0 ** -23).all())
