@@ -56,7 +56,7 @@ __device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
 // without the value scales in the maximum: the plain formula. For the few rows that the f16
 // probabilities cannot resolve (see kResolved), so simple rather than fast: a lane per key for the
 // scores, a lane per D / 32 columns for the sum. (All rows of 128 requests of up to 4096 tokens, 32 / 8
-// heads of 128: 10 ms, where the kernel takes 0.12.) With `look`, leaves a row alone, and returns
+// heads of 128: 3.3 ms, where the kernel takes 0.12.) With `look`, leaves a row alone, and returns
 // false, if all the values it sees are zero: its 0 is right already (a cache of zeros: 0.7 ms).
 // Pages' value scales may differ by up to 2^100 (beyond, the kernels' fp32 denominators lose keys
 // that still count).
@@ -77,8 +77,10 @@ __device__ __forceinline__ bool exact_row(const Params& p, int b, int h, const _
   for (int k0 = 0; k0 < keys && !any; k0 += 32) {
     const int64_t row = k0 + lane < keys ? row_of(k0 + lane) : -1;
     uint32_t bits = 0;
-    for (int c = 0; c < D / 16 && row >= 0; ++c) {
-      const uint4 x = __ldg(reinterpret_cast<const uint4*>(p.v_codes + row * D) + c);
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) {
+      const uint4 x = row >= 0 ? __ldg(reinterpret_cast<const uint4*>(p.v_codes + row * D) + c)
+                               : make_uint4(0, 0, 0, 0);
       bits |= x.x | x.y | x.z | x.w;
     }
     any = __any_sync(0xffffffffu, (bits & (INT8 ? 0xffffffffu : 0x7f7f7f7fu)) != 0);
@@ -95,15 +97,23 @@ __device__ __forceinline__ bool exact_row(const Params& p, int b, int h, const _
     const float vs = row >= 0 ? __ldg(p.v_scale + (row >> p.page_shift)) : 0.f;
     float s = 0.f;
 #pragma unroll 1
-    for (int c = 0; c < D / 4; ++c) {
-      uint32_t f[2];
-      kv::decode4<INT8>(row >= 0 ? __ldg(reinterpret_cast<const uint32_t*>(p.k_codes + row * D) + c) : 0u,
-                        f[0], f[1]);
+    for (int c0 = 0; c0 < D; c0 += 64) {       // 64 codes in flight
+      uint4 x4[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 k2 = kv::f16x2_to_float2(f[e >> 1]);
-        const float qd = __shfl_sync(0xffffffffu, qv[e % kCols], (c * 4 + e) / kCols);
-        s = fmaf(qd, (e & 1 ? k2.y : k2.x) * ks, s);
+      for (int c = 0; c < 4; ++c)
+        x4[c] = row >= 0 ? __ldg(reinterpret_cast<const uint4*>(p.k_codes + row * D + c0) + c)
+                         : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int c = 0; c < 16; ++c) {
+        const uint32_t w4[4] = {x4[c / 4].x, x4[c / 4].y, x4[c / 4].z, x4[c / 4].w};
+        uint32_t f[2];
+        kv::decode4<INT8>(w4[c % 4], f[0], f[1]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 k2 = kv::f16x2_to_float2(f[e >> 1]);
+          const float qd = __shfl_sync(0xffffffffu, qv[e % kCols], (c0 + c * 4 + e) / kCols);
+          s = fmaf(qd, (e & 1 ? k2.y : k2.x) * ks, s);
+        }
       }
     }
     s = row >= 0 ? s * p.scale_log2 : -INFINITY;
@@ -114,19 +124,26 @@ __device__ __forceinline__ bool exact_row(const Params& p, int b, int h, const _
 #pragma unroll
     for (int i = 0; i < kCols; ++i) x[i] *= down;
 #pragma unroll 1
-    for (int k = 0; k < min(32, keys - k0); ++k) {
-      const int64_t at = __shfl_sync(0xffffffffu, row, k);
-      if (at < 0) continue;
-      const float wk = __shfl_sync(0xffffffffu, w, k), sk = __shfl_sync(0xffffffffu, vs, k);
-      const uint8_t* codes = p.v_codes + at * D + lane * kCols;
-      const uint32_t raw = kCols == 4 ? __ldg(reinterpret_cast<const uint32_t*>(codes))
-                                      : __ldg(reinterpret_cast<const uint16_t*>(codes));
-      uint32_t f[2];
-      kv::decode4<INT8>(raw, f[0], f[1]);
+    for (int k = 0; k < min(32, keys - k0); k += 8) {
+      uint32_t raw[8];
 #pragma unroll
-      for (int i = 0; i < kCols; ++i) {
-        const float2 v2 = kv::f16x2_to_float2(f[i >> 1]);
-        x[i] = fmaf(wk, (i & 1 ? v2.y : v2.x) * sk, x[i]);
+      for (int i = 0; i < 8; ++i) {            // a missing page or none: weight 0, codes 0
+        const int64_t at = __shfl_sync(0xffffffffu, row, k + i);
+        const uint8_t* codes = p.v_codes + at * D + lane * kCols;
+        raw[i] = at < 0 ? 0u
+                        : kCols == 4 ? __ldg(reinterpret_cast<const uint32_t*>(codes))
+                                     : __ldg(reinterpret_cast<const uint16_t*>(codes));
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float wk = __shfl_sync(0xffffffffu, w, k + i), sk = __shfl_sync(0xffffffffu, vs, k + i);
+        uint32_t f[2];
+        kv::decode4<INT8>(raw[i], f[0], f[1]);
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) {
+          const float2 v2 = kv::f16x2_to_float2(f[c >> 1]);
+          x[c] = fmaf(wk, (c & 1 ? v2.y : v2.x) * sk, x[c]);
+        }
       }
     }
   }
